@@ -31,6 +31,9 @@ enum mt_status {
 /* Output element types of the GEMM entry points. */
 enum mt_dtype { MT_BF16 = 0, MT_F32 = 1 };
 
+/* Activations of the gated projection: g / (1 + e^-g), and the tanh form of gelu. */
+enum mt_activation { MT_ACT_SILU = 0, MT_ACT_GELU = 1 };
+
 /* Flags of mt_quantize_nvfp4 / mt_amax_bf16. */
 enum mt_quantize_flags {
   MT_Q_2D = 1,       /* one scale per 16x16 block, shared by both copies */
@@ -348,6 +351,66 @@ int mt_peer_gather(const void* const* shared, int n, int me, const int64_t* src_
  * raised to max |out|. */
 int mt_peer_reduce_bf16(const void* stage, int n, int64_t rows, int64_t cols, void* out, float* amax_out,
                         mt_stream_t stream);
+
+/* ---- Around the linear layers of a transformer block (no counterpart in the reference, whose
+ * LayerNormLinear is unfused, miniTransformer/module/layernorm_linear.py:299-306) ---- */
+
+/* Residual addition and root-mean-square norm of rows:
+ *   h = bf16(x + residual), rstd = 1 / sqrt(mean(h^2) + eps), y = bf16(h * rstd * gamma)
+ * x, residual: bf16 [rows, cols], row strides in elements (multiples of 8); cols a multiple of 8, at most
+ * 32768. residual may be null: then h is x, and the h output must be null. gamma: bf16 or fp32
+ * (gamma_dtype). Outputs, each optional (h required with a residual), rows contiguous:
+ *   h bf16; rstd fp32 [rows]; y bf16; amax device fp32 scalar, raised to max |y| (zeroed by the caller);
+ *   q, s (stride s_stride), s_swz: MXFP8 copy of y as mt_quantize_mxfp8 makes it (cols % 32 == 0).
+ * h may be the same buffer as x or residual. */
+int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
+                       const void* gamma, int gamma_dtype, int64_t rows, int64_t cols, float eps,
+                       void* h, float* rstd, void* y, float* amax,
+                       uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz, mt_stream_t stream);
+
+/* Gradients of mt_rmsnorm_forward with respect to h (= x and residual alike) and gamma:
+ *   dx = rstd * (dy * gamma - xhat * mean(dy * gamma * xhat)) + dres, dgamma = sum over rows of dy * xhat,
+ *   xhat = h * rstd.
+ * dres (optional): gradient that reaches h from elsewhere. dx bf16 [rows, cols] contiguous, may be dres's
+ * buffer; dgamma fp32 [cols], overwritten, the same bits for the same inputs on the same device.
+ * workspace: mt_rmsnorm_backward_workspace(rows, cols) bytes (for the current device). */
+int64_t mt_rmsnorm_backward_workspace(int64_t rows, int64_t cols);
+int mt_rmsnorm_backward(const void* dy, int64_t dy_stride, const void* h, int64_t h_stride,
+                        const void* gamma, int gamma_dtype, const float* rstd, const void* dres, int64_t dres_stride,
+                        int64_t rows, int64_t cols, void* dx, float* dgamma,
+                        void* workspace, int64_t workspace_bytes, mt_stream_t stream);
+
+/* Gated projection of a feed-forward block: [g | u] = alpha * x W^T with W = [W_gate; W_up] of 2F rows,
+ * h = bf16(act(g) * u), computed from the fp32 products in one kernel. Operands, scales and alpha
+ * as in mt_gemm_mxfp8 / mt_gemm_nvfp4 (x [M, K], w [2F, K]; K % 32 == 0); F % 32 == 0. sw_swz covers all
+ * 2F rows; when F is not a multiple of 128 the rows of W_up start inside a 128-row chunk of it,
+ * and sw_up_swz gives their scales in a GEMM layout of their own (F rows), otherwise it may be null.
+ * Outputs (struct below, each optional, at least one of h, gu, q; 32-byte aligned, rows contiguous):
+ *   h   bf16 [M, F]            gu  bf16 [M, 2F], the projections (what mt_gated_backward reads)
+ *   q, s, s_stride, s_swz      MXFP8 copy of h as mt_quantize_mxfp8 makes it
+ *   amax                       device fp32 scalar, raised to max |h| (zeroed by the caller) */
+typedef struct mt_gated_outputs {
+  void* h;
+  void* gu;
+  uint8_t* q;
+  uint8_t* s;
+  int64_t s_stride;
+  uint8_t* s_swz;
+  float* amax;
+} mt_gated_outputs;
+int mt_gemm_gated_mxfp8(const uint8_t* x, const uint8_t* sx_swz, const uint8_t* w, const uint8_t* sw_swz,
+                        const uint8_t* sw_up_swz, int64_t M, int64_t F, int64_t K, int activation,
+                        const mt_gated_outputs* out, mt_stream_t stream);
+int mt_gemm_gated_nvfp4(const uint8_t* x, const uint8_t* sx_swz, const float* amax_x,
+                        const uint8_t* w, const uint8_t* sw_swz, const uint8_t* sw_up_swz, const float* amax_w,
+                        int64_t M, int64_t F, int64_t K, int activation,
+                        const mt_gated_outputs* out, mt_stream_t stream);
+
+/* Gradient of h = act(g) * u: du = bf16(dh * act(g)), dg = bf16(dh * u * act'(g)).
+ * dh bf16 [rows, F] (row stride dh_stride), gu bf16 [rows, 2F] = [g | u]; F % 32 == 0.
+ * dgu bf16 [rows, 2F] = [dg | du]; amax (optional): device fp32 scalar, raised to max |dgu|. */
+int mt_gated_backward(const void* dh, int64_t dh_stride, const void* gu, int64_t rows, int64_t F, int activation,
+                      void* dgu, float* amax, mt_stream_t stream);
 
 /* Reads and clears the device-side status word the kernels raise when a bounded wait
  * expires (0 = clean). Synchronises the given stream. */

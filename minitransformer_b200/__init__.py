@@ -3,6 +3,7 @@
 Public surface (same names as the reference package):
     minitransformer_b200.module.linear.Linear
     minitransformer_b200.module.group_linear.GroupedLinear
+    minitransformer_b200.module.rmsnorm.RMSNorm, minitransformer_b200.module.gated_linear.GatedLinear
     minitransformer_b200.module.config   (QLinearParams, QuantizeRecipe, ...)
     minitransformer_b200.ops.quantization (QuantizeOpBase, QParams, MMParams, ...)
     minitransformer_b200.kernels          (torch front end of the C ABI in include/mt_b200.h)
@@ -12,7 +13,7 @@ import sys
 
 __version__ = "0.1.0"
 
-_ALIASED = ("module", "module.linear", "module.group_linear", "module.config", "module.base", "module._common",
+_ALIASED = ("module", "module.linear", "module.group_linear", "module.rmsnorm", "module.gated_linear", "module.config", "module.base", "module._common",
             "ops", "ops.quantization", "ops.nvfp4_quantize_op", "ops.mxfp8_quantize_op",
             "distributed", "distributed.distributed", "utils", "utils.utils")
 

@@ -13,6 +13,7 @@ HEADER_PATHS = (os.path.join(INCLUDE_DIR, "mt_b200.h"), os.path.join(INCLUDE_DIR
 
 MT_BF16, MT_F32 = 0, 1
 MT_Q_2D, MT_Q_RHT, MT_Q_ROWPAD16, MT_Q_AMAX_ZEROED = 1, 2, 4, 8
+MT_ACT_SILU, MT_ACT_GELU = 0, 1
 MT_MAX_PEERS, MT_PEER_CTRL_BYTES, MT_IPC_HANDLE_BYTES = 8, 4096, 64
 
 _c = ctypes
@@ -26,6 +27,14 @@ class GemmOpts(ctypes.Structure):
 
 
 _opts = _c.POINTER(GemmOpts)
+
+
+class GatedOutputs(ctypes.Structure):
+    """mt_gated_outputs of include/mt_b200.h."""
+    _fields_ = [("h", _vp), ("gu", _vp), ("q", _vp), ("s", _vp), ("s_stride", _i64), ("s_swz", _vp), ("amax", _vp)]
+
+
+_gated = _c.POINTER(GatedOutputs)
 
 _SIGNATURES = {
     "mt_version": (_int, []),
@@ -65,6 +74,13 @@ _SIGNATURES = {
     "mt_peer_gather": (_int, [_c.POINTER(_vp), _int, _int, _c.POINTER(_i64), _c.POINTER(_vp), _c.POINTER(_i64), _int, _int,
                               _int, _vp]),
     "mt_peer_reduce_bf16": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
+    "mt_rmsnorm_forward": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _c.c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _i64, _vp, _vp]),
+    "mt_rmsnorm_backward_workspace": (_i64, [_i64, _i64]),
+    "mt_rmsnorm_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "mt_gemm_gated_mxfp8": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _gated, _vp]),
+    "mt_gemm_gated_nvfp4": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _gated, _vp]),
+    "mt_gated_backward": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "mt_read_device_status": (_int, [_c.POINTER(_int), _vp]),
 }
 

@@ -1,0 +1,596 @@
+// Gated projection for sm_100a: h = act(x Wg^T) * (x Wu^T) from block-scaled operands (MXFP8 or
+// NVFP4, K-major), both products, the activation and the product of the two in one kernel.
+//
+//   [g | u] = alpha * x W^T, W = [Wg; Wu] of 2F rows          fp32 in tensor memory
+//   h = bf16(act(g) * u)                                      from the fp32 accumulators
+//   on request: bf16 [g | u] (what the backward pass reads), E4M3 codes + E8M0 scales of h by rows
+//   (bit for bit mt_quantize_mxfp8 of h), max |h|
+//
+// Two kernels, by the number of rows M of x:
+//
+// gemm_gated_rows_kernel (M <= 128, decoding): the weights are read once and dominate, so they
+// take the 128-row side of the MMA and the tokens the column side (N = M rounded up to 32):
+// the tensor time shrinks with M and the pipeline holds almost only weight bytes. A CTA owns 128
+// features; its accumulators [128 features x tokens] put one feature in each lane, so a warp
+// owns one 1x32 block of h for every token.
+//
+// gemm_gated_pair_kernel (M > 128): a CTA pair (cta_group::2) per 256 rows x 128 features. The B
+// tile of 256 rows is [128 rows of Wg; 128 rows of Wu], one half loaded by either CTA, so g and u
+// of a feature end up 128 accumulator columns apart in the same lane.
+//
+// Every wait on an mbarrier is bounded, as in the plain GEMM kernels.
+#include <algorithm>
+
+#include "gated_act.cuh"
+#include "gemm_common.cuh"
+#include "quantize_common.cuh"
+
+namespace mt {
+
+struct GatedArgs {
+  const uint8_t *sa, *sb_gate, *sb_up;   // scale factors, chunk layout
+  int64_t kc;                            // chunks per 128-row block (all operands share K)
+  int64_t M, F, K_bytes;
+  const float *amax_a, *amax_b;
+  int* status;
+  int act;
+  // outputs, each optional
+  __nv_bfloat16 *h, *gu;
+  float* amax;
+  uint8_t *q, *s, *s_swz;
+  int64_t s_stride, kc_h;                // kc_h: chunks per 128-row block of s_swz
+  int tiles_m, tiles_n, num_tiles;
+};
+
+__device__ __forceinline__ float gated_alpha(const GatedArgs& a) {
+  return a.amax_a != nullptr ? __fdiv_rn(__fmul_rn(*a.amax_a, *a.amax_b), 6.0f * 6.0f * 448.0f * 448.0f) : 1.0f;
+}
+
+__device__ __forceinline__ float gated_act_any(int act, float g) {
+  return act == MT_ACT_SILU ? gated_act<MT_ACT_SILU>(g) : gated_act<MT_ACT_GELU>(g);
+}
+
+// ------------------------------------------------------------------------------------------
+// M <= 128
+// ------------------------------------------------------------------------------------------
+template <int kFormat, int BT, int STAGES>
+struct GatedRowsCfg {
+  static constexpr int CH = (kFormat == FMT_NVFP4) ? 4 : 1;
+  static constexpr int W_BYTES = 128 * G_BLOCK_KB;       // one projection's rows of a stage
+  static constexpr int T_BYTES = BT * G_BLOCK_KB;        // tokens of a stage
+  static constexpr int SF_BYTES = CH * 512;
+  static constexpr int STAGE_BYTES = 2 * W_BYTES + T_BYTES + 3 * SF_BYTES;
+  static constexpr int OFF_G = 0;
+  static constexpr int OFF_U = STAGES * W_BYTES;
+  static constexpr int OFF_T = 2 * STAGES * W_BYTES;
+  static constexpr int OFF_SF = OFF_T + STAGES * T_BYTES;   // [gate | up | tokens] chunks per stage
+  static constexpr int OFF_BAR = OFF_SF + STAGES * 3 * SF_BYTES;
+  static constexpr int NUM_BARS = 2 * STAGES + 1;
+  static constexpr int SMEM_ALLOC = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
+  static constexpr int TMEM_G = 0, TMEM_U = BT;
+  static constexpr int TMEM_SF = 2 * BT;                 // gate, up, tokens: 4 * CH columns each
+  static constexpr int TMEM_COLS = (2 * BT + 12 * CH <= 128) ? 128 : (2 * BT + 12 * CH <= 256) ? 256 : 512;
+  static_assert(2 * BT + 12 * CH <= 512, "tensor memory over-subscribed");
+  static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory over-subscribed");
+};
+
+// One CTA per 128 features. 192 threads: TMA producer warp, MMA warp, four epilogue warps.
+template <int kFormat, int BT, int STAGES>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    gemm_gated_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
+                           const __grid_constant__ CUtensorMap map_u, const GatedArgs a) {
+  using Cfg = GatedRowsCfg<kFormat, BT, STAGES>;
+  constexpr int CH = Cfg::CH;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + STAGES;
+  uint64_t* acc_full = bars + 2 * STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NUM_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x;
+  const int64_t f0 = (int64_t)tile * 128;
+  const int num_k = (int)((a.K_bytes + G_BLOCK_KB - 1) / G_BLOCK_KB);
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_g);
+    prefetch_tensormap(&map_u);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int k = 0; k < num_k; ++k) {
+        if (!mbar_wait_bounded(&empty_bar[s], ph ^ 1, abort_flag, a.status, DS_EMPTY_WAIT)) break;
+        mbar_expect_tx(&full_bar[s], Cfg::STAGE_BYTES);
+        tma_load_2d(smem + Cfg::OFF_G + s * Cfg::W_BYTES, &map_g, &full_bar[s], k * G_BLOCK_KB, (int32_t)f0);
+        tma_load_2d(smem + Cfg::OFF_U + s * Cfg::W_BYTES, &map_u, &full_bar[s], k * G_BLOCK_KB, (int32_t)f0);
+        tma_load_2d(smem + Cfg::OFF_T + s * Cfg::T_BYTES, &map_x, &full_bar[s], k * G_BLOCK_KB, 0);
+        uint8_t* sf = smem + Cfg::OFF_SF + s * 3 * Cfg::SF_BYTES;
+        const int64_t chunk = (int64_t)tile * a.kc + (int64_t)k * CH;
+        bulk_load_1d(sf, a.sb_gate + chunk * 512, Cfg::SF_BYTES, &full_bar[s]);
+        bulk_load_1d(sf + Cfg::SF_BYTES, a.sb_up + chunk * 512, Cfg::SF_BYTES, &full_bar[s]);
+        bulk_load_1d(sf + 2 * Cfg::SF_BYTES, a.sa + (int64_t)k * CH * 512, Cfg::SF_BYTES, &full_bar[s]);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool alive = true;
+      const uint32_t sm = smem_u32(smem);
+      for (int k = 0; k < num_k; ++k) {
+        if (!mbar_wait_bounded(&full_bar[s], ph, abort_flag, a.status, DS_TMA_WAIT)) { alive = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < 3 * CH; ++i)
+          tc_copy_sf(tmem_base + Cfg::TMEM_SF + 4 * i, umma_desc_sf(sm + Cfg::OFF_SF + s * 3 * Cfg::SF_BYTES + i * 512));
+        const uint64_t gdesc = umma_desc_sw128(sm + Cfg::OFF_G + s * Cfg::W_BYTES);
+        const uint64_t udesc = umma_desc_sw128(sm + Cfg::OFF_U + s * Cfg::W_BYTES);
+        const uint64_t tdesc = umma_desc_sw128(sm + Cfg::OFF_T + s * Cfg::T_BYTES);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t idesc = make_idesc(kFormat, BT, j);
+          const uint32_t sf = tmem_base + Cfg::TMEM_SF + (kFormat == FMT_NVFP4 ? 4 * j : 0);
+          const uint32_t acc = (k > 0 || j > 0) ? 1u : 0u;
+          issue_mma<kFormat>(tmem_base + Cfg::TMEM_G, gdesc + 2 * j, tdesc + 2 * j, idesc, sf, sf + 8 * CH, acc);
+          issue_mma<kFormat>(tmem_base + Cfg::TMEM_U, udesc + 2 * j, tdesc + 2 * j, idesc, sf + 4 * CH, sf + 8 * CH, acc);
+        }
+        tc_commit(&empty_bar[s]);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+      if (alive) tc_commit(acc_full);
+    }
+    __syncwarp();
+  } else {
+    // epilogue: lane <-> feature, warp <-> one 1x32 block of h per token
+    const int qd = warp & 3;
+    const float alpha = gated_alpha(a);
+    const int64_t f = f0 + qd * 32 + lane;
+    const bool f_ok = f < a.F;
+    const int kb = (int)(f0 >> 5) + qd;
+    AmaxAcc am;
+    if (mbar_wait_bounded(acc_full, 0, abort_flag, a.status, DS_ACC_FULL_WAIT)) {
+      tc_fence_after();
+      const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(qd * 32) << 16);
+      uint8_t* chunk = a.s_swz + (int64_t)tile * 512;   // tokens of one 128-row block, blocks 4 tile ..
+#pragma unroll 1
+      for (int c = 0; c < BT; c += 32) {
+        if (c >= a.M) break;
+        uint32_t g[32], u[32];
+        tc_ld_32x32(lane_base + Cfg::TMEM_G + c, g);
+        tc_ld_32x32(lane_base + Cfg::TMEM_U + c, u);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int64_t t = c + i;
+          if (t >= a.M) break;
+          const float gv = alpha * __uint_as_float(g[i]), uv = alpha * __uint_as_float(u[i]);
+          const __nv_bfloat16 hb = __float2bfloat16_rn(gated_act_any(a.act, gv) * uv);
+          const float hv = __bfloat162float(hb);
+          if (f_ok) {
+            if (a.h != nullptr) a.h[t * a.F + f] = hb;
+            if (a.gu != nullptr) {
+              a.gu[t * 2 * a.F + f] = __float2bfloat16_rn(gv);
+              a.gu[t * 2 * a.F + a.F + f] = __float2bfloat16_rn(uv);
+            }
+            am.f = fmaxf(am.f, fabsf(hv));
+          }
+          if (a.q != nullptr) {
+            // bit patterns of non-negative floats order like integers; a NaN is dropped as in mt_quantize_mxfp8
+            const float av = fmaxf(fabsf(hv), 0.0f);
+            const int e = e8m0_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, f_ok ? __float_as_uint(av) : 0u)));
+            if (f_ok) a.q[t * a.F + f] = __nv_cvt_float_to_fp8(hv * exp2_neg(e), __NV_SATFINITE, __NV_E4M3);
+            if (lane == 0) {
+              const uint8_t sb = static_cast<uint8_t>(e + 127);
+              if (f_ok && a.s != nullptr) a.s[t * a.s_stride + kb] = sb;
+              if (a.s_swz != nullptr) chunk[sf_chunk_offset((int)t, kb)] = f_ok ? sb : 0;
+            }
+          }
+        }
+      }
+      if (a.s_swz != nullptr) {   // rows without a token, and the chunks up to the padded count
+        for (int t = (int)a.M + lane; t < 128; t += 32) chunk[sf_chunk_offset(t, kb)] = 0;
+        if (tile == a.tiles_n - 1)
+          for (int64_t i = (a.tiles_n * 512) / 16 + qd * 32 + lane; i < a.kc_h * 32; i += 128)
+            *reinterpret_cast<uint4*>(a.s_swz + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+      if (a.amax != nullptr) amax_publish(a.amax, am, lane);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// M > 128
+// ------------------------------------------------------------------------------------------
+constexpr int GP_EPI_WARPS = 8;
+constexpr int GP_THREADS = 64 + 32 * GP_EPI_WARPS;
+
+template <int kFormat, int STAGES>
+struct GatedPairCfg {
+  static constexpr int CH = (kFormat == FMT_NVFP4) ? 4 : 1;
+  static constexpr int A_BYTES = 128 * G_BLOCK_KB;
+  static constexpr int B_BYTES = 128 * G_BLOCK_KB;       // this CTA's projection: gate (rank 0) or up (rank 1)
+  static constexpr int SF_BYTES = CH * 512;              // x rows of this CTA; gate and up: both CTAs load both
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + 3 * SF_BYTES;
+  static constexpr int OFF_A = 0;
+  static constexpr int OFF_B = STAGES * A_BYTES;
+  static constexpr int OFF_SF = OFF_B + STAGES * B_BYTES;   // [x | gate | up] per stage
+  static constexpr int OFF_BAR = OFF_SF + STAGES * 3 * SF_BYTES;
+  static constexpr int NUM_BARS = 2 * STAGES + 2;
+  static constexpr int SMEM_ALLOC = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
+  static constexpr int TMEM_SFA = 256;
+  static constexpr int TMEM_SFB = TMEM_SFA + 4 * CH;
+  static_assert(TMEM_SFB + 8 * CH <= G_TMEM_COLS, "tensor memory over-subscribed");
+  static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory over-subscribed");
+};
+
+// 32 features of one row: bf16 h (and bf16 g, u) -> global memory, codes and scale byte.
+template <int kAct>
+__device__ __forceinline__ void gated_store_block(const GatedArgs& a, const uint32_t (&g)[32], const uint32_t (&u)[32],
+                                                  float alpha, int64_t row, int64_t f, bool row_ok, AmaxAcc& am) {
+  const bool ok = row_ok && f < a.F;    // F is a multiple of 32: a block is whole or absent
+  uint32_t hw[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float g0 = alpha * __uint_as_float(g[2 * i]), g1 = alpha * __uint_as_float(g[2 * i + 1]);
+    const float u0 = alpha * __uint_as_float(u[2 * i]), u1 = alpha * __uint_as_float(u[2 * i + 1]);
+    hw[i] = f32x2_to_bf16x2(pack2(gated_act<kAct>(g0) * u0, gated_act<kAct>(g1) * u1));
+  }
+  if (ok && a.gu != nullptr) {
+    __nv_bfloat16* pg = a.gu + row * 2 * a.F + f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t wg[8], wu[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = 16 * half + 2 * i;
+        wg[i] = f32x2_to_bf16x2(pack2(alpha * __uint_as_float(g[c]), alpha * __uint_as_float(g[c + 1])));
+        wu[i] = f32x2_to_bf16x2(pack2(alpha * __uint_as_float(u[c]), alpha * __uint_as_float(u[c + 1])));
+      }
+      st_global_v8(pg + 16 * half, wg);
+      st_global_v8(pg + a.F + 16 * half, wu);
+    }
+  }
+  if (ok && a.h != nullptr) {
+    __nv_bfloat16* ph = a.h + row * a.F + f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t w[8] = {hw[8 * half], hw[8 * half + 1], hw[8 * half + 2], hw[8 * half + 3],
+                             hw[8 * half + 4], hw[8 * half + 5], hw[8 * half + 6], hw[8 * half + 7]};
+      st_global_v8(ph + 16 * half, w);
+    }
+  }
+  if (a.amax == nullptr && a.q == nullptr) return;
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = absmax2(m, hw[i]);
+  if (ok) amax_bf16x2(am, m);
+  if (a.q == nullptr) return;
+  const int e = e8m0_exponent(absmax2_to_float(m));
+  const float enc = exp2_neg(e);
+  const f32x2_t enc2 = pack2(enc, enc);
+  uint32_t cw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) cw[i] = e4m3x4_from_words(hw[2 * i], hw[2 * i + 1], enc2);
+  if (ok) st_global_v8(a.q + row * a.F + f, cw);
+  const uint8_t sb = ok ? static_cast<uint8_t>(e + 127) : 0;
+  const int64_t kb = f >> 5;
+  if (ok && a.s != nullptr) a.s[row * a.s_stride + kb] = sb;
+  if (a.s_swz != nullptr && (row >> 7) < (a.M + 127) / 128)
+    a.s_swz[((row >> 7) * a.kc_h + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)kb)] = sb;
+}
+
+template <int kFormat, int STAGES, int kAct>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_THREADS, 1)
+    gemm_gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
+                           const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_sx,
+                           const __grid_constant__ CUtensorMap map_sg, const __grid_constant__ CUtensorMap map_su,
+                           const GatedArgs a) {
+  using Cfg = GatedPairCfg<kFormat, STAGES>;
+  constexpr int CH = Cfg::CH;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* full_bar = bars;                  // leader only, signalled by both CTAs' loads
+  uint64_t* empty_bar = bars + STAGES;        // per CTA, signalled by the leader's commit
+  uint64_t* acc_full = bars + 2 * STAGES;     // per CTA, signalled by the leader's commit
+  uint64_t* acc_empty = bars + 2 * STAGES + 1;   // leader only: 2 x GP_EPI_WARPS arrivals
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NUM_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int num_k = (int)((a.K_bytes + G_BLOCK_KB - 1) / G_BLOCK_KB);
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * GP_EPI_WARPS);
+    mbar_fence_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(rank == 0 ? &map_g : &map_u);
+    prefetch_tensormap(&map_sx);
+    prefetch_tensormap(&map_sg);
+    prefetch_tensormap(&map_su);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, G_TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();      // both CTAs' barriers exist before either signals the other
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool alive = true;
+      const CUtensorMap* map_w = rank == 0 ? &map_g : &map_u;
+      for (int tile = pair; tile < a.num_tiles && alive; tile += num_pairs) {
+        const int mb = tile / a.tiles_n, nb = tile - mb * a.tiles_n;
+        const int32_t x_row = mb * 256 + (int)rank * 128, w_row = nb * 128;
+        const int32_t sx_chunk = (int32_t)((2 * mb + (int)rank) * a.kc), sw_chunk = (int32_t)(nb * a.kc);
+        for (int k = 0; k < num_k; ++k) {
+          if (!mbar_wait_bounded(&empty_bar[s], ph ^ 1, abort_flag, a.status, DS_EMPTY_WAIT)) { alive = false; break; }
+          if (leader) mbar_expect_tx(&full_bar[s], 2 * Cfg::STAGE_BYTES);
+          const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
+          tma_load_2d_pair(smem + Cfg::OFF_A + s * Cfg::A_BYTES, &map_x, bar, k * G_BLOCK_KB, x_row);
+          tma_load_2d_pair(smem + Cfg::OFF_B + s * Cfg::B_BYTES, map_w, bar, k * G_BLOCK_KB, w_row);
+          uint8_t* sf = smem + Cfg::OFF_SF + s * 3 * Cfg::SF_BYTES;
+          tma_load_2d_pair(sf, &map_sx, bar, 0, sx_chunk + k * CH);
+          tma_load_2d_pair(sf + Cfg::SF_BYTES, &map_sg, bar, 0, sw_chunk + k * CH);
+          tma_load_2d_pair(sf + 2 * Cfg::SF_BYTES, &map_su, bar, 0, sw_chunk + k * CH);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader && elect_one()) {
+      int s = 0;
+      uint32_t ph = 0, tile_it = 0;
+      bool alive = true;
+      const uint32_t sm = smem_u32(smem);
+      for (int tile = pair; tile < a.num_tiles && alive; tile += num_pairs, ++tile_it) {
+        if (!mbar_wait_bounded(acc_empty, (tile_it & 1) ^ 1, abort_flag, a.status, DS_ACC_EMPTY_WAIT)) { alive = false; break; }
+        tc_fence_after();
+        for (int k = 0; k < num_k; ++k) {
+          if (!mbar_wait_bounded(&full_bar[s], ph, abort_flag, a.status, DS_TMA_WAIT)) { alive = false; break; }
+          tc_fence_after();
+          const uint32_t sf = sm + Cfg::OFF_SF + s * 3 * Cfg::SF_BYTES;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) tc_copy_sf_pair(tmem_base + Cfg::TMEM_SFA + 4 * c, umma_desc_sf(sf + c * 512));
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+              tc_copy_sf_pair(tmem_base + Cfg::TMEM_SFB + 4 * (2 * c + p), umma_desc_sf(sf + ((1 + p) * CH + c) * 512));
+          const uint64_t adesc = umma_desc_sw128(sm + Cfg::OFF_A + s * Cfg::A_BYTES);
+          const uint64_t bdesc = umma_desc_sw128(sm + Cfg::OFF_B + s * Cfg::B_BYTES);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t idesc = make_idesc_pair(kFormat, 256, j);
+            issue_mma_pair<kFormat>(tmem_base, adesc + 2 * j, bdesc + 2 * j, idesc,
+                                    tmem_base + Cfg::TMEM_SFA + (kFormat == FMT_NVFP4 ? 4 * j : 0),
+                                    tmem_base + Cfg::TMEM_SFB + (kFormat == FMT_NVFP4 ? 8 * j : 0), (k > 0 || j > 0) ? 1u : 0u);
+          }
+          tc_commit_pair(&empty_bar[s], 3);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+        if (alive) tc_commit_pair(acc_full, 3);
+      }
+    }
+    __syncwarp();
+  } else {
+    // epilogue: a warp reads the lane quarter warp % 4 and 64 of the 128 features
+    const int e = warp - 2, qd = warp & 3, half = (e >> 2) & 1;
+    const float alpha = gated_alpha(a);
+    const uint32_t acc_empty_leader = map_to_cta(smem_u32(acc_empty), 0);
+    uint32_t tile_it = 0;
+    AmaxAcc am;
+    for (int tile = pair; tile < a.num_tiles; tile += num_pairs, ++tile_it) {
+      const int mb = tile / a.tiles_n, nb = tile - mb * a.tiles_n;
+      if (!mbar_wait_bounded(acc_full, tile_it & 1, abort_flag, a.status, DS_ACC_FULL_WAIT)) break;
+      tc_fence_after();
+      const uint32_t tm = tmem_base + (static_cast<uint32_t>(qd * 32) << 16) + half * 64;
+      // the whole block goes to registers and tensor memory back to the MMA issuer at once
+      uint32_t g[2][32], u[2][32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        tc_ld_32x32(tm + c * 32, g[c]);
+        tc_ld_32x32(tm + 128 + c * 32, u[c]);
+      }
+      tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty_leader);
+      const int64_t row = (int64_t)mb * 256 + rank * 128 + qd * 32 + lane;
+      const int64_t f = (int64_t)nb * 128 + half * 64;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) gated_store_block<kAct>(a, g[c], u[c], alpha, row, f + c * 32, row < a.M, am);
+      if (a.s_swz != nullptr && nb == a.tiles_n - 1 && half == 0 && (row >> 7) < (a.M + 127) / 128) {
+        // this row's words in the chunks up to the padded count
+        uint8_t* cell = a.s_swz + (row >> 7) * a.kc_h * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+        for (int64_t c = a.tiles_n; c < a.kc_h; ++c) *reinterpret_cast<uint32_t*>(cell + c * 512) = 0u;
+      }
+    }
+    if (a.amax != nullptr) amax_publish(a.amax, am, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  // neither CTA may exit (or free tensor memory) while its peer can still touch it
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, G_TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------
+template <int kFormat, int BT, int STAGES>
+static int launch_gated_rows(const CUtensorMap& mx, const CUtensorMap& mg, const CUtensorMap& mu, const GatedArgs& a,
+                             cudaStream_t st) {
+  using Cfg = GatedRowsCfg<kFormat, BT, STAGES>;
+  auto kern = gemm_gated_rows_kernel<kFormat, BT, STAGES>;
+  static bool attr_set[MT_MAX_DEVICES] = {};
+  const int slot = current_device_slot();
+  if (!attr_set[slot]) {
+    MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC));
+    attr_set[slot] = true;
+  }
+  MT_CUDA(launch_pdl(kern, dim3(a.tiles_n), dim3(G_THREADS), (size_t)Cfg::SMEM_ALLOC, st, mx, mg, mu, a));
+  return MT_OK;
+}
+
+template <int kFormat, int STAGES, int kAct>
+static int launch_gated_pair(const CUtensorMap (&m)[6], const GatedArgs& a, cudaStream_t st) {
+  using Cfg = GatedPairCfg<kFormat, STAGES>;
+  auto kern = gemm_gated_pair_kernel<kFormat, STAGES, kAct>;
+  static int max_pairs_dev[MT_MAX_DEVICES] = {};   // 0 = not yet queried on that device
+  int& max_pairs = max_pairs_dev[current_device_slot()];
+  if (max_pairs <= 0) {
+    MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC));
+    int dev = 0, sms = 0;
+    MT_CUDA(cudaGetDevice(&dev));
+    MT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms / 2 * 2);
+    cfg.blockDim = dim3(GP_THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM_ALLOC;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) { cudaGetLastError(); n = sms / 2; }
+    max_pairs = n;
+  }
+  const int pairs = std::min(a.num_tiles, max_pairs);
+  MT_CUDA(launch_pdl(kern, dim3(2 * pairs), dim3(GP_THREADS), (size_t)Cfg::SMEM_ALLOC, st, m[0], m[1], m[2], m[3], m[4], m[5], a));
+  return MT_OK;
+}
+
+template <int kFormat>
+static int launch_gated(const uint8_t* x, const uint8_t* wg, const uint8_t* wu, GatedArgs& a, cudaStream_t st) {
+  CUtensorMap m[6];
+  const uint64_t ld = (uint64_t)a.K_bytes;
+  constexpr uint32_t CH = kFormat == FMT_NVFP4 ? 4 : 1;
+  const bool small = a.M <= 128;
+  const uint32_t bt = small ? (uint32_t)((a.M + 31) / 32 * 32) : 128u;
+  int rc = make_tensor_map_2d(&m[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, ld, (uint64_t)a.M, ld, G_BLOCK_KB, bt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == MT_OK) rc = make_tensor_map_2d(&m[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wg, ld, (uint64_t)a.F, ld, G_BLOCK_KB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == MT_OK) rc = make_tensor_map_2d(&m[2], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wu, ld, (uint64_t)a.F, ld, G_BLOCK_KB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != MT_OK) return rc;
+  a.tiles_n = (int)((a.F + 127) / 128);
+  if (small) {
+    if (bt == 32) return launch_gated_rows<kFormat, 32, 5>(m[0], m[1], m[2], a, st);
+    if (bt == 64) return launch_gated_rows<kFormat, 64, 4>(m[0], m[1], m[2], a, st);
+    if (bt == 96) return launch_gated_rows<kFormat, 96, 4>(m[0], m[1], m[2], a, st);
+    return launch_gated_rows<kFormat, 128, 4>(m[0], m[1], m[2], a, st);
+  }
+  const uint64_t rb_x = (uint64_t)((a.M + 127) / 128), rb_w = (uint64_t)((a.F + 127) / 128);
+  rc = make_tensor_map_2d(&m[3], CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.sa, 128, rb_x * a.kc, 512, 128, CH, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc == MT_OK) rc = make_tensor_map_2d(&m[4], CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.sb_gate, 128, rb_w * a.kc, 512, 128, CH, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc == MT_OK) rc = make_tensor_map_2d(&m[5], CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.sb_up, 128, rb_w * a.kc, 512, 128, CH, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc != MT_OK) return rc;
+  a.tiles_m = (int)((a.M + 255) / 256);
+  a.num_tiles = a.tiles_m * a.tiles_n;
+  constexpr int ST = kFormat == FMT_NVFP4 ? 5 : 6;
+  return a.act == MT_ACT_SILU ? launch_gated_pair<kFormat, ST, MT_ACT_SILU>(m, a, st)
+                              : launch_gated_pair<kFormat, ST, MT_ACT_GELU>(m, a, st);
+}
+
+static int gemm_gated(int format, const uint8_t* x, const uint8_t* sx, const float* amax_x, const uint8_t* w,
+                      const uint8_t* sw, const uint8_t* sw_up, const float* amax_w, int64_t M, int64_t F, int64_t K,
+                      const mt_gated_outputs* out, int act, cudaStream_t st) {
+  const char* name = format == FMT_NVFP4 ? "mt_gemm_gated_nvfp4" : "mt_gemm_gated_mxfp8";
+  MT_REQUIRE(M >= 0 && F >= 0 && K >= 0, "%s: negative shape", name);
+  MT_REQUIRE(M < (int64_t)1 << 30 && F < (int64_t)1 << 28 && K < (int64_t)1 << 30, "%s: shape out of range", name);
+  MT_REQUIRE(gated_act_known(act), "%s: activation %d not supported", name, act);
+  MT_REQUIRE(out != nullptr, "%s: null outputs", name);
+  MT_REQUIRE(K > 0 && K % 32 == 0, "%s: K (%lld) must be a positive multiple of 32", name, (long long)K);
+  MT_REQUIRE(F % 32 == 0, "%s: F (%lld) must be a multiple of 32", name, (long long)F);
+  if (M == 0 || F == 0) return MT_OK;
+  MT_REQUIRE(x && sx && w && sw, "%s: null pointer", name);
+  MT_REQUIRE(sw_up || F % 128 == 0, "%s: with F (%lld) not a multiple of 128 the scales of the second projection must be "
+             "given apart, in a layout of their own", name, (long long)F);
+  MT_REQUIRE(aligned16(x) && aligned16(sx) && aligned16(w) && aligned16(sw) && aligned16(sw_up),
+             "%s: operands must be 16-byte aligned", name);
+  if (format == FMT_NVFP4) MT_REQUIRE(amax_x && amax_w, "%s: per-tensor abs-max pointers are required", name);
+  MT_REQUIRE(out->h || out->gu || out->q, "%s: no output requested", name);
+  const uintptr_t align = reinterpret_cast<uintptr_t>(out->h) | reinterpret_cast<uintptr_t>(out->gu) | reinterpret_cast<uintptr_t>(out->q);
+  MT_REQUIRE((align & 31) == 0, "%s: outputs must be 32-byte aligned", name);
+  MT_REQUIRE(aligned16(out->s_swz), "%s: swizzled scale buffer must be 16-byte aligned", name);
+  MT_REQUIRE(!out->q || (out->s && out->s_stride >= F / 32), "%s: codes need s with a stride of at least F / 32", name);
+  MT_REQUIRE(out->q || (!out->s && !out->s_swz), "%s: scales without codes", name);
+  const int64_t block = format == FMT_NVFP4 ? 16 : 32;
+  GatedArgs a{};
+  a.M = M; a.F = F;
+  a.K_bytes = format == FMT_NVFP4 ? K / 2 : K;
+  a.kc = ((K / block + 3) / 4 + 3) / 4 * 4;
+  a.sa = sx; a.sb_gate = sw; a.sb_up = sw_up ? sw_up : sw + F / 128 * a.kc * 512;
+  a.amax_a = format == FMT_NVFP4 ? amax_x : nullptr;
+  a.amax_b = format == FMT_NVFP4 ? amax_w : nullptr;
+  a.act = act;
+  a.h = static_cast<__nv_bfloat16*>(out->h); a.gu = static_cast<__nv_bfloat16*>(out->gu); a.amax = out->amax;
+  a.q = out->q; a.s = out->s; a.s_swz = out->s_swz; a.s_stride = out->s_stride;
+  a.kc_h = ((F / 32 + 3) / 4 + 3) / 4 * 4;
+  a.status = device_status_ptr();
+  if (!a.status) return fail(MT_ERR_CUDA, "device status word not reachable");
+  const uint8_t* wu = w + F * a.K_bytes;
+  return format == FMT_NVFP4 ? launch_gated<FMT_NVFP4>(x, w, wu, a, st) : launch_gated<FMT_MXFP8>(x, w, wu, a, st);
+}
+
+}  // namespace mt
+
+extern "C" int mt_gemm_gated_mxfp8(const uint8_t* x, const uint8_t* sx_swz, const uint8_t* w, const uint8_t* sw_swz,
+                                   const uint8_t* sw_up_swz, int64_t M, int64_t F, int64_t K, int activation,
+                                   const mt_gated_outputs* out, mt_stream_t stream) {
+  return mt::gemm_gated(mt::FMT_MXFP8, x, sx_swz, nullptr, w, sw_swz, sw_up_swz, nullptr, M, F, K, out, activation,
+                        static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mt_gemm_gated_nvfp4(const uint8_t* x, const uint8_t* sx_swz, const float* amax_x, const uint8_t* w,
+                                   const uint8_t* sw_swz, const uint8_t* sw_up_swz, const float* amax_w, int64_t M,
+                                   int64_t F, int64_t K, int activation, const mt_gated_outputs* out, mt_stream_t stream) {
+  return mt::gemm_gated(mt::FMT_NVFP4, x, sx_swz, amax_x, w, sw_swz, sw_up_swz, amax_w, M, F, K, out, activation,
+                        static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,366 @@
+// Residual addition + root-mean-square norm, with the MXFP8 copy of the result, and its gradient.
+//
+//   h = bf16(x + r)                     (h = x without a residual)
+//   rstd = 1 / sqrt(mean_k h_k^2 + eps) fp32, from the rounded h: what the next layer adds to and
+//                                       what the backward pass reads again
+//   y = bf16(h * rstd * gamma)          products in fp32, rounded once
+//   copy: E4M3 codes and E8M0 scales of y in 1x32 blocks, bit for bit what mt_quantize_mxfp8 makes of y
+//
+// Both directions move every element once and do a few operations on it: they are bound by HBM
+// (forward with residual and codes: 2 + 2 read, 2 + 1 written per element; backward 2 + 2 (+ 2)
+// read, 2 written).
+#include "quantize_common.cuh"
+
+namespace mt {
+
+constexpr int RN_MAX_COLS = 32768;
+
+struct RmsNormArgs {
+  const __nv_bfloat16 *x, *r;
+  int64_t x_stride, r_stride;
+  const void* gamma;
+  int gamma_f32;
+  int64_t rows, cols;
+  float eps;
+  __nv_bfloat16* h;
+  float* rstd;
+  __nv_bfloat16* y;
+  float* amax;
+  uint8_t *q, *s, *s_swz;
+  int64_t s_stride, kc;
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Sum over the CTA, the same value (and the same order of additions) in every thread. `slot` holds
+// 32 floats; callers that reduce twice alternate between two of them.
+__device__ __forceinline__ float block_sum(float v, float* slot) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  v = warp_sum(v);
+  if (lane == 0) slot[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < warps ? slot[lane] : 0.0f);
+}
+
+// Eight consecutive gammas as fp32.
+__device__ __forceinline__ void load_gamma8(const void* gamma, int is_f32, int64_t col, float (&g)[8]) {
+  if (is_f32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(gamma) + col);
+    const float4 a = __ldg(p), b = __ldg(p + 1);
+    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w; g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+  } else {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(gamma) + col));
+    g[0] = bf16_lo(a.x); g[1] = bf16_hi(a.x); g[2] = bf16_lo(a.y); g[3] = bf16_hi(a.y);
+    g[4] = bf16_lo(a.z); g[5] = bf16_hi(a.z); g[6] = bf16_lo(a.w); g[7] = bf16_hi(a.w);
+  }
+}
+
+// One CTA per row, V vectors of 8 columns per thread (vector i * blockDim + thread). The row stays
+// in registers between the sum and the scaling. A 1x32 block is four adjacent lanes. CTAs
+// beyond the last row fill the padding of the GEMM-layout scales with zeros.
+template <int V>
+__global__ void __launch_bounds__(1024) rmsnorm_rows_kernel(const RmsNormArgs a) {
+  __shared__ float slot[32];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
+  pdl_trigger();
+  pdl_wait();
+  if (row >= a.rows) {
+    uint8_t* cell = a.s_swz + (row >> 7) * a.kc * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+    for (int64_t c = tid; c < a.kc; c += blockDim.x) *reinterpret_cast<uint32_t*>(cell + c * 512) = 0u;
+    return;
+  }
+  uint4 w[V];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (v < nvec) {
+      w[i] = *reinterpret_cast<const uint4*>(a.x + row * a.x_stride + (int64_t)v * 8);
+      if (a.r != nullptr) {
+        const uint4 r = *reinterpret_cast<const uint4*>(a.r + row * a.r_stride + (int64_t)v * 8);
+        w[i].x = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].x), bf16x2_to_f32x2(r.x)));
+        w[i].y = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].y), bf16x2_to_f32x2(r.y)));
+        w[i].z = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].z), bf16x2_to_f32x2(r.z)));
+        w[i].w = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].w), bf16x2_to_f32x2(r.w)));
+        if (a.h != nullptr) *reinterpret_cast<uint4*>(a.h + row * a.cols + (int64_t)v * 8) = w[i];
+      }
+    }
+    const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ss = fmaf(bf16_lo(ws[j]), bf16_lo(ws[j]), ss);
+      ss = fmaf(bf16_hi(ws[j]), bf16_hi(ws[j]), ss);
+    }
+  }
+  ss = block_sum(ss, slot);
+  const float rstd = __frsqrt_rn(__fdiv_rn(ss, (float)a.cols) + a.eps);
+  if (tid == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
+
+  uint32_t am = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    const bool on = v < nvec;
+    float g[8];
+    uint32_t yw[4] = {0, 0, 0, 0};
+    if (on) {
+      load_gamma8(a.gamma, a.gamma_f32, (int64_t)v * 8, g);
+      const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      const f32x2_t r2 = pack2(rstd, rstd);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        yw[j] = f32x2_to_bf16x2(mul2(mul2(bf16x2_to_f32x2(ws[j]), r2), pack2(g[2 * j], g[2 * j + 1])));
+      if (a.y != nullptr)
+        *reinterpret_cast<uint4*>(a.y + row * a.cols + (int64_t)v * 8) = make_uint4(yw[0], yw[1], yw[2], yw[3]);
+    }
+    uint32_t m = absmax2(absmax2(yw[0], yw[1]), absmax2(yw[2], yw[3]));
+    am = absmax2(am, m);
+    if (a.q != nullptr) {
+      m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const int e = e8m0_exponent(absmax2_to_float(m));
+      if (on) {
+        const float enc = exp2_neg(e);
+        const f32x2_t enc2 = pack2(enc, enc);
+        *reinterpret_cast<uint2*>(a.q + row * a.cols + (int64_t)v * 8) =
+            make_uint2(e4m3x4_from_words(yw[0], yw[1], enc2), e4m3x4_from_words(yw[2], yw[3], enc2));
+        if ((v & 3) == 0) {
+          const int kb = v >> 2;
+          a.s[row * a.s_stride + kb] = static_cast<uint8_t>(e + 127);
+          if (a.s_swz != nullptr)
+            a.s_swz[((row >> 7) * a.kc + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), kb)] = static_cast<uint8_t>(e + 127);
+        }
+      }
+    }
+  }
+  if (a.s_swz != nullptr)   // blocks beyond the row, up to the padded chunk count
+    for (int64_t kb = (a.cols >> 5) + tid; kb < a.kc * 4; kb += blockDim.x)
+      a.s_swz[((row >> 7) * a.kc + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)kb)] = 0;
+  if (a.amax != nullptr) {
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
+    if ((tid & 31) == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
+  }
+}
+
+// ---- gradient ----
+//   a = dy * gamma, xhat = h * rstd
+//   dx = rstd * (a - xhat * mean_k(a * xhat)) (+ dres),   dgamma = sum_rows dy * xhat
+struct RmsNormGradArgs {
+  const __nv_bfloat16 *dy, *h, *dres;
+  int64_t dy_stride, h_stride, dres_stride;
+  const void* gamma;
+  int gamma_f32;
+  const float* rstd;
+  int64_t rows, cols;
+  __nv_bfloat16* dx;
+  float* partial;   // [gridDim.x, cols]
+};
+
+// Persistent CTAs over rows; a thread keeps the same columns for every row, so the column sums
+// of dgamma stay in its registers and are written once per CTA. The partial sums are then added
+// in a fixed order (rmsnorm_dgamma_kernel): the result does not depend on scheduling.
+template <int V>
+__global__ void __launch_bounds__(1024) rmsnorm_grad_kernel(const RmsNormGradArgs a) {
+  __shared__ float slot[2][32];
+  const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
+  pdl_trigger();
+  pdl_wait();
+  float acc[V][8];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    uint4 dy[V], h[V];
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = i * blockDim.x + tid;
+      dy[i] = h[i] = make_uint4(0, 0, 0, 0);
+      if (v < nvec) {
+        dy[i] = *reinterpret_cast<const uint4*>(a.dy + row * a.dy_stride + (int64_t)v * 8);
+        h[i] = *reinterpret_cast<const uint4*>(a.h + row * a.h_stride + (int64_t)v * 8);
+      }
+    }
+    const float rstd = a.rstd[row];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = i * blockDim.x + tid;
+      if (v >= nvec) continue;
+      float g[8];
+      load_gamma8(a.gamma, a.gamma_f32, (int64_t)v * 8, g);
+      const uint32_t d[4] = {dy[i].x, dy[i].y, dy[i].z, dy[i].w}, x[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dot = fmaf(bf16_lo(d[j]) * g[2 * j], bf16_lo(x[j]), dot);
+        dot = fmaf(bf16_hi(d[j]) * g[2 * j + 1], bf16_hi(x[j]), dot);
+      }
+    }
+    dot = block_sum(dot, slot[turn]);
+    // xhat * mean(a * xhat) = h * rstd * (rstd * dot / cols)
+    const float c = rstd * rstd * __fdiv_rn(dot, (float)a.cols);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = i * blockDim.x + tid;
+      if (v >= nvec) continue;
+      float g[8];
+      load_gamma8(a.gamma, a.gamma_f32, (int64_t)v * 8, g);
+      uint4 rs = make_uint4(0, 0, 0, 0);
+      if (a.dres != nullptr) rs = *reinterpret_cast<const uint4*>(a.dres + row * a.dres_stride + (int64_t)v * 8);
+      const uint32_t d[4] = {dy[i].x, dy[i].y, dy[i].z, dy[i].w}, x[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+      const uint32_t r[4] = {rs.x, rs.y, rs.z, rs.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float d0 = bf16_lo(d[j]), d1 = bf16_hi(d[j]), x0 = bf16_lo(x[j]), x1 = bf16_hi(x[j]);
+        const float o0 = fmaf(rstd, fmaf(d0, g[2 * j], -x0 * c), bf16_lo(r[j]));
+        const float o1 = fmaf(rstd, fmaf(d1, g[2 * j + 1], -x1 * c), bf16_hi(r[j]));
+        o[j] = f32x2_to_bf16x2(pack2(o0, o1));
+        acc[i][2 * j] = fmaf(d0, x0 * rstd, acc[i][2 * j]);
+        acc[i][2 * j + 1] = fmaf(d1, x1 * rstd, acc[i][2 * j + 1]);
+      }
+      *reinterpret_cast<uint4*>(a.dx + row * a.cols + (int64_t)v * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    if (v >= nvec) continue;
+    float4* p = reinterpret_cast<float4*>(a.partial + (int64_t)blockIdx.x * a.cols + (int64_t)v * 8);
+    p[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    p[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+  }
+}
+
+// dgamma[k] = sum of `parts` partial rows, in order. 32 columns per CTA, 8 row groups.
+__global__ void __launch_bounds__(256) rmsnorm_dgamma_kernel(const float* partial, int parts, int64_t cols, float* dgamma) {
+  __shared__ float sum[8][32];
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+  pdl_trigger();
+  pdl_wait();
+  float v = 0.0f;
+  if (col < cols)
+    for (int p = grp; p < parts; p += 8) v += partial[(int64_t)p * cols + col];
+  sum[grp][lane] = v;
+  __syncthreads();
+  if (grp == 0 && col < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += sum[i][lane];
+    dgamma[col] = v;
+  }
+}
+
+static int rn_sm_count() {
+  static int n[MT_MAX_DEVICES] = {};
+  const int slot = current_device_slot();
+  if (n[slot] == 0) {
+    int dev = 0, c = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
+    n[slot] = c > 0 ? c : 148;
+  }
+  return n[slot];
+}
+
+// Threads per row for V vectors per thread.
+static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / V + 31) / 32 * 32); }
+
+static int rn_grad_ctas(int64_t rows) {
+  const int64_t most = 2 * (int64_t)rn_sm_count();
+  return (int)(rows < most ? rows : most);
+}
+
+static bool row_aligned(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
+
+}  // namespace mt
+
+extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* residual, int64_t r_stride, const void* gamma,
+                                  int gamma_dtype, int64_t rows, int64_t cols, float eps, void* h, float* rstd, void* y,
+                                  float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz,
+                                  mt_stream_t stream) {
+  using namespace mt;
+  const char* name = "mt_rmsnorm_forward";
+  MT_REQUIRE(rows >= 0 && cols > 0 && cols <= RN_MAX_COLS, "%s: cols (%lld) must be within [1, %d]", name, (long long)cols, RN_MAX_COLS);
+  MT_REQUIRE(cols % 8 == 0, "%s: cols (%lld) must be a multiple of 8", name, (long long)cols);
+  MT_REQUIRE(gamma_dtype == MT_BF16 || gamma_dtype == MT_F32, "%s: gamma dtype %d not supported", name, gamma_dtype);
+  MT_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", name);
+  MT_REQUIRE(rows < (int64_t)1 << 31, "%s: too many rows", name);
+  if (rows == 0) return MT_OK;
+  MT_REQUIRE(x && gamma, "%s: null x / gamma", name);
+  MT_REQUIRE(x_stride >= cols && row_aligned(x, x_stride), "%s: x needs 16-byte aligned rows", name);
+  MT_REQUIRE(!residual || (r_stride >= cols && row_aligned(residual, r_stride)), "%s: residual needs 16-byte aligned rows", name);
+  MT_REQUIRE(!residual || h, "%s: a residual needs an output for the sum", name);
+  MT_REQUIRE(residual || !h, "%s: without a residual there is no sum to write", name);
+  MT_REQUIRE(aligned16(gamma) && aligned16(h) && aligned16(y), "%s: pointers must be 16-byte aligned", name);
+  if (q) {
+    MT_REQUIRE(cols % 32 == 0, "%s: cols (%lld) must be a multiple of 32 for the MXFP8 copy", name, (long long)cols);
+    MT_REQUIRE(s && s_stride >= cols / 32, "%s: the MXFP8 copy needs s with a stride of at least cols / 32", name);
+    MT_REQUIRE(aligned16(q) && aligned16(s_swz), "%s: q and s_swz must be 16-byte aligned", name);
+  } else {
+    MT_REQUIRE(!s && !s_swz, "%s: scales without codes", name);
+  }
+  RmsNormArgs a{};
+  a.x = static_cast<const __nv_bfloat16*>(x); a.x_stride = x_stride;
+  a.r = static_cast<const __nv_bfloat16*>(residual); a.r_stride = r_stride;
+  a.gamma = gamma; a.gamma_f32 = gamma_dtype == MT_F32;
+  a.rows = rows; a.cols = cols; a.eps = eps;
+  a.h = static_cast<__nv_bfloat16*>(h); a.rstd = rstd; a.y = static_cast<__nv_bfloat16*>(y); a.amax = amax;
+  a.q = q; a.s = s; a.s_swz = s_swz; a.s_stride = s_stride;
+  a.kc = ((cols / 32 + 3) / 4 + 3) / 4 * 4;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)(s_swz ? (rows + 127) / 128 * 128 : rows));
+  if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<1>, grid, dim3(rn_threads(cols, 1)), 0, st, a));
+  else if (cols <= 16384) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<2>, grid, dim3(rn_threads(cols, 2)), 0, st, a));
+  else MT_CUDA(launch_pdl(rmsnorm_rows_kernel<4>, grid, dim3(rn_threads(cols, 4)), 0, st, a));
+  return MT_OK;
+}
+
+extern "C" int64_t mt_rmsnorm_backward_workspace(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return (int64_t)mt::rn_grad_ctas(rows) * cols * 4;
+}
+
+extern "C" int mt_rmsnorm_backward(const void* dy, int64_t dy_stride, const void* h, int64_t h_stride, const void* gamma,
+                                   int gamma_dtype, const float* rstd, const void* dres, int64_t dres_stride, int64_t rows,
+                                   int64_t cols, void* dx, float* dgamma, void* workspace, int64_t workspace_bytes,
+                                   mt_stream_t stream) {
+  using namespace mt;
+  const char* name = "mt_rmsnorm_backward";
+  MT_REQUIRE(rows >= 0 && cols > 0 && cols <= RN_MAX_COLS, "%s: cols (%lld) must be within [1, %d]", name, (long long)cols, RN_MAX_COLS);
+  MT_REQUIRE(cols % 8 == 0, "%s: cols (%lld) must be a multiple of 8", name, (long long)cols);
+  MT_REQUIRE(gamma_dtype == MT_BF16 || gamma_dtype == MT_F32, "%s: gamma dtype %d not supported", name, gamma_dtype);
+  MT_REQUIRE(dgamma && aligned16(dgamma), "%s: dgamma must be given, 16-byte aligned", name);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {   // no rows: the sum over them is zero
+    MT_CUDA(cudaMemsetAsync(dgamma, 0, (size_t)cols * 4, st));
+    return MT_OK;
+  }
+  MT_REQUIRE(dy && h && gamma && rstd && dx, "%s: null pointer", name);
+  MT_REQUIRE(dy_stride >= cols && row_aligned(dy, dy_stride) && h_stride >= cols && row_aligned(h, h_stride),
+             "%s: dy and h need 16-byte aligned rows", name);
+  MT_REQUIRE(!dres || (dres_stride >= cols && row_aligned(dres, dres_stride)), "%s: dres needs 16-byte aligned rows", name);
+  MT_REQUIRE(aligned16(gamma) && aligned16(dx), "%s: pointers must be 16-byte aligned", name);
+  MT_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= mt_rmsnorm_backward_workspace(rows, cols),
+             "%s: workspace of %lld bytes is too small (mt_rmsnorm_backward_workspace)", name, (long long)workspace_bytes);
+  RmsNormGradArgs a{};
+  a.dy = static_cast<const __nv_bfloat16*>(dy); a.dy_stride = dy_stride;
+  a.h = static_cast<const __nv_bfloat16*>(h); a.h_stride = h_stride;
+  a.dres = static_cast<const __nv_bfloat16*>(dres); a.dres_stride = dres_stride;
+  a.gamma = gamma; a.gamma_f32 = gamma_dtype == MT_F32; a.rstd = rstd;
+  a.rows = rows; a.cols = cols;
+  a.dx = static_cast<__nv_bfloat16*>(dx); a.partial = static_cast<float*>(workspace);
+  const int ctas = rn_grad_ctas(rows);
+  if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_grad_kernel<1>, dim3(ctas), dim3(rn_threads(cols, 1)), 0, st, a));
+  else if (cols <= 16384) MT_CUDA(launch_pdl(rmsnorm_grad_kernel<2>, dim3(ctas), dim3(rn_threads(cols, 2)), 0, st, a));
+  else MT_CUDA(launch_pdl(rmsnorm_grad_kernel<4>, dim3(ctas), dim3(rn_threads(cols, 4)), 0, st, a));
+  MT_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st,
+                     static_cast<const float*>(workspace), ctas, cols, dgamma));
+  return MT_OK;
+}

@@ -1,6 +1,7 @@
 """Thin torch-tensor front end over the C-ABI kernels: allocates outputs with torch, passes
 raw pointers and the current CUDA stream, raises on any error. No arithmetic happens here."""
 import contextlib
+import functools
 import threading
 from dataclasses import dataclass
 from typing import Optional
@@ -505,6 +506,248 @@ def grouped_wgrad_mxfp8(qa_t, sa_t_swz, qb_t, sb_t_swz, m_splits, *, out_dtype=t
               int(accumulate), _stream())
     _count(1)
     return out
+
+
+# ---- around the linear layers: norm, gated projection ----
+def _on_tensor_device(fn):
+    """Runs fn with the device of its first argument current, so that launches and allocations go
+    there whatever device is current in the caller."""
+    @functools.wraps(fn)
+    def wrapper(first, *args, **kw):
+        _require_cuda(first, "the first argument")
+        if first.device.index == torch.cuda.current_device():
+            return fn(first, *args, **kw)
+        with torch.cuda.device(first.device):
+            return fn(first, *args, **kw)
+    return wrapper
+
+
+def _same_device(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise _lib.MtError(f"{name} is on {t.device}, expected {first.device}")
+
+
+def _rows(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
+    """A bf16 matrix whose rows the kernels can read (16-byte aligned, unit column stride), copied only
+    when its own layout is not like that."""
+    if t.dtype != torch.bfloat16 or t.dim() != 2:
+        raise _lib.MtError(f"{name} must be a 2-D bf16 tensor, got {tuple(t.shape)} {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise _lib.MtError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.numel() and (t.stride(1) != 1 or t.stride(0) < t.shape[1] or t.stride(0) % 8 or t.data_ptr() % 16):
+        # (clone: a one-row or one-column slice may call itself contiguous and still start off a 16-byte address)
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride for the C ABI (that of a single row is of no account and may be anything)."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _gamma(weight: torch.Tensor, cols: int) -> torch.Tensor:
+    if weight.dim() != 1 or weight.shape[0] != cols:
+        raise _lib.MtError(f"the norm's weight has shape {tuple(weight.shape)}, expected ({cols},)")
+    if weight.dtype not in (torch.bfloat16, torch.float32):
+        raise _lib.MtError(f"the norm's weight must be bf16 or fp32, got {weight.dtype}")
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    return weight
+
+
+def _amax_scalar(device) -> torch.Tensor:
+    """A device scalar holding 0, to be raised to an abs-max."""
+    z = _zeroed_scalars(device, 1)
+    return torch.zeros(1, dtype=torch.float32, device=device) if z is None else z
+
+
+@dataclass
+class RmsNormResult:
+    """h: x + residual in bf16 (x itself without a residual); rstd fp32 [rows]; y bf16 or None; quantized:
+    MXFP8 copies of y or None; amax: max |y| or None."""
+    h: torch.Tensor
+    rstd: torch.Tensor
+    y: Optional[torch.Tensor] = None
+    quantized: Optional[Quantized] = None
+    amax: Optional[torch.Tensor] = None
+
+
+@_on_tensor_device
+def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: Optional[torch.Tensor] = None,
+            want_y: bool = True, quantize: bool = True, return_transpose: bool = True,
+            want_amax: bool = False) -> RmsNormResult:
+    """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight over the rows of x [rows, cols] (bf16).
+    quantize: also the MXFP8 copies of y (cols % 32 == 0), row-wise and, with return_transpose, transposed,
+    bit for bit those of quantize_mxfp8(y). want_y=False leaves y out when only the copies are used."""
+    _same_device(x, weight=weight, residual=residual)
+    x = _rows(x, "x")
+    M, C = x.shape
+    if residual is not None:
+        residual = _rows(residual, "residual", (M, C))
+    weight = _gamma(weight, C)
+    if not (want_y or quantize):
+        raise _lib.MtError("rmsnorm: neither y nor its MXFP8 copies requested")
+    dev, u8 = x.device, torch.uint8
+    return_transpose = return_transpose and quantize
+    h = x if residual is None else torch.empty((M, C), dtype=torch.bfloat16, device=dev)
+    rstd = torch.empty(M, dtype=torch.float32, device=dev)
+    y = torch.empty((M, C), dtype=torch.bfloat16, device=dev) if want_y or return_transpose else None
+    amax = _amax_scalar(dev) if want_amax else None
+    q = s = s_swz = None
+    if quantize and not return_transpose:
+        q = torch.empty((M, C), dtype=u8, device=dev)
+        s = torch.empty((M, C // 32), dtype=u8, device=dev)
+        s_swz = torch.empty(swizzled_scale_bytes(M, C // 32), dtype=u8, device=dev)
+    _lib.call("mt_rmsnorm_forward", x.data_ptr(), _row_stride(x), _ptr(residual), 0 if residual is None else _row_stride(residual),
+              weight.data_ptr(), _out_dtype_code(weight.dtype), M, C, eps, None if residual is None else h.data_ptr(),
+              rstd.data_ptr(), _ptr(y), _ptr(amax), _ptr(q), _ptr(s), C // 32, _ptr(s_swz), _stream())
+    _count(1 if M else 0)
+    quantized = None
+    if return_transpose:
+        quantized = quantize_mxfp8(y, return_transpose=True)
+    elif quantize:
+        quantized = Quantized(q, s, s_swz)
+    return RmsNormResult(h, rstd, y if want_y else None, quantized, amax)
+
+
+@_on_tensor_device
+def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, *,
+                     dresidual: Optional[torch.Tensor] = None):
+    """Gradients of rmsnorm: (dx bf16, dweight fp32), dx with respect to x and to the residual alike.
+    h and rstd as rmsnorm returned them; dresidual: gradient that reaches h from elsewhere, added to dx."""
+    _same_device(dy, h=h, weight=weight, rstd=rstd, dresidual=dresidual)
+    dy = _rows(dy, "dy")
+    M, C = dy.shape
+    h = _rows(h, "h", (M, C))
+    weight = _gamma(weight, C)
+    if rstd.dtype != torch.float32 or rstd.shape != (M,) or not rstd.is_contiguous():
+        raise _lib.MtError(f"rstd must be a contiguous fp32 tensor of {M} values")
+    if dresidual is not None:
+        dresidual = _rows(dresidual, "dresidual", (M, C))
+    dx = torch.empty((M, C), dtype=torch.bfloat16, device=dy.device)
+    dweight = torch.empty(C, dtype=torch.float32, device=dy.device)
+    n = int(_lib.load().mt_rmsnorm_backward_workspace(M, C))
+    work = torch.empty(n, dtype=torch.uint8, device=dy.device) if n else None
+    _lib.call("mt_rmsnorm_backward", dy.data_ptr(), _row_stride(dy), h.data_ptr(), _row_stride(h), weight.data_ptr(),
+              _out_dtype_code(weight.dtype), rstd.data_ptr(), _ptr(dresidual),
+              0 if dresidual is None else _row_stride(dresidual), M, C, dx.data_ptr(), dweight.data_ptr(), _ptr(work), n,
+              _stream())
+    _count(2 if M else 0)
+    return dx, dweight
+
+
+_ACTIVATIONS = {"silu": _lib.MT_ACT_SILU, "gelu": _lib.MT_ACT_GELU}
+
+
+def _activation_code(name: str) -> int:
+    if name not in _ACTIVATIONS:
+        raise _lib.MtError(f"activation {name!r} is not supported ({', '.join(sorted(_ACTIVATIONS))})")
+    return _ACTIVATIONS[name]
+
+
+@dataclass
+class GatedResult:
+    """h bf16 [M, F]; gu bf16 [M, 2F]: the projections [g | u]; quantized: row-wise MXFP8 copy of h; amax: max |h|
+    (each None unless requested)."""
+    h: Optional[torch.Tensor] = None
+    gu: Optional[torch.Tensor] = None
+    quantized: Optional[Quantized] = None
+    amax: Optional[torch.Tensor] = None
+
+
+def _gemm_gated(fmt, qa, sa_swz, amax_a, qb, sb_swz, amax_b, activation, sb_lin, want_h, want_gu, quantize_h, want_amax):
+    _same_device(qa, sa_swz=sa_swz, qb=qb, sb_swz=sb_swz, amax_a=amax_a, amax_b=amax_b, sb_lin=sb_lin)
+    act = _activation_code(activation)
+    if qa.dim() != 2 or qb.dim() != 2 or qa.shape[1] != qb.shape[1] or qb.shape[0] % 2:
+        raise _lib.MtError(f"gated projection of {tuple(qa.shape)} with {tuple(qb.shape)}: operands are codes [M, K] and [2F, K]")
+    if qa.dtype != torch.uint8 or qb.dtype != torch.uint8 or not qa.is_contiguous() or not qb.is_contiguous():
+        raise _lib.MtError("gated projection: operands must be contiguous uint8 codes")
+    M, F = qa.shape[0], qb.shape[0] // 2
+    K = qa.shape[1] * (2 if fmt == "nvfp4" else 1)
+    block = 16 if fmt == "nvfp4" else 32
+    if sa_swz.numel() < swizzled_scale_bytes(M, K // block) or sb_swz.numel() < swizzled_scale_bytes(2 * F, K // block):
+        raise _lib.MtError("gated projection: scale buffers are smaller than the GEMM layout of the operands")
+    if not (want_h or want_gu or quantize_h):
+        raise _lib.MtError("gated projection: no output requested")
+    sb_up = None
+    if F % 128 and F:
+        # the second projection's rows start inside a 128-row chunk of the stacked scales: a layout of their own
+        if sb_lin is None or sb_lin.shape[0] < 2 * F:
+            raise _lib.MtError(f"gated projection: F = {F} is not a multiple of 128, which needs the row-major weight scales (sb_lin)")
+        sb_up = swizzle_scales(sb_lin[F:2 * F])
+    dev, u8 = qa.device, torch.uint8
+    r = GatedResult()
+    o = _lib.GatedOutputs()
+    if want_h:
+        r.h = torch.empty((M, F), dtype=torch.bfloat16, device=dev)
+        o.h = r.h.data_ptr()
+    if want_gu:
+        r.gu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dev)
+        o.gu = r.gu.data_ptr()
+    if want_amax:
+        r.amax = _amax_scalar(dev)
+        o.amax = r.amax.data_ptr()
+    if quantize_h:
+        q = torch.empty((M, F), dtype=u8, device=dev)
+        s = torch.empty((M, F // 32), dtype=u8, device=dev)
+        s_swz = torch.empty(swizzled_scale_bytes(M, F // 32), dtype=u8, device=dev)
+        r.quantized = Quantized(q, s, s_swz)
+        o.q, o.s, o.s_stride, o.s_swz = q.data_ptr(), s.data_ptr(), F // 32, s_swz.data_ptr()
+    _count(1 if M and F else 0)
+    if fmt == "mxfp8":
+        _lib.call("mt_gemm_gated_mxfp8", qa.data_ptr(), sa_swz.data_ptr(), qb.data_ptr(), sb_swz.data_ptr(), _ptr(sb_up), M, F, K,
+                  act, _lib.ctypes.byref(o), _stream())
+    else:
+        _lib.call("mt_gemm_gated_nvfp4", qa.data_ptr(), sa_swz.data_ptr(), amax_a.data_ptr(), qb.data_ptr(), sb_swz.data_ptr(),
+                  _ptr(sb_up), amax_b.data_ptr(), M, F, K, act, _lib.ctypes.byref(o), _stream())
+    return r
+
+
+@_on_tensor_device
+def gemm_gated_mxfp8(qa, sa_swz, qb, sb_swz, *, activation: str = "silu", sb_lin=None, want_h: bool = True,
+                     want_gu: bool = False, quantize_h: bool = False, want_amax: bool = False) -> GatedResult:
+    """h = act(x Wg^T) * (x Wu^T) in one kernel: qa codes of x [M, K], qb codes of [Wg; Wu] [2F, K] (K and F
+    multiples of 32), scales in the GEMM layout. sb_lin: the weight's row-major scales, needed when F is not
+    a multiple of 128. Outputs as requested: h, the projections gu, the row-wise MXFP8 copy of h, max |h|."""
+    return _gemm_gated("mxfp8", qa, sa_swz, None, qb, sb_swz, None, activation, sb_lin, want_h, want_gu, quantize_h, want_amax)
+
+
+@_on_tensor_device
+def gemm_gated_nvfp4(qa, sa_swz, amax_a, qb, sb_swz, amax_b, *, activation: str = "silu", sb_lin=None, want_h: bool = True,
+                     want_gu: bool = False, quantize_h: bool = False, want_amax: bool = False) -> GatedResult:
+    """gemm_gated_mxfp8 on NVFP4 operands (packed codes [M, K / 2] and [2F, K / 2], per-tensor abs-max)."""
+    return _gemm_gated("nvfp4", qa, sa_swz, amax_a, qb, sb_swz, amax_b, activation, sb_lin, want_h, want_gu, quantize_h, want_amax)
+
+
+@dataclass
+class GatedGradResult:
+    """Gradient [dg | du] of the gated projection's two products: dgu in bf16, or its MXFP8 copies, and max |dgu|."""
+    dgu: Optional[torch.Tensor] = None
+    quantized: Optional[Quantized] = None
+    amax: Optional[torch.Tensor] = None
+
+
+@_on_tensor_device
+def gated_backward(dh: torch.Tensor, gu: torch.Tensor, *, activation: str = "silu", quantize: bool = True,
+                   want_dgu: bool = False, want_amax: bool = False) -> GatedGradResult:
+    """From dh [M, F] and the projections gu [M, 2F] = [g | u] (bf16): du = dh act(g), dg = dh u act'(g).
+    quantize: MXFP8 copies of [dg | du], row-wise and transposed, bit for bit those of quantize_mxfp8 of the
+    bf16 gradient; want_dgu: the bf16 gradient itself."""
+    _same_device(dh, gu=gu)
+    act = _activation_code(activation)
+    dh = _rows(dh, "dh")
+    M, F = dh.shape
+    gu = _rows(gu, "gu", (M, 2 * F))
+    if not gu.is_contiguous():
+        gu = gu.contiguous()
+    if not (quantize or want_dgu):
+        raise _lib.MtError("gated_backward: neither the gradient nor its MXFP8 copies requested")
+    amax = _amax_scalar(dh.device) if want_amax else None
+    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dh.device)
+    _lib.call("mt_gated_backward", dh.data_ptr(), _row_stride(dh), gu.data_ptr(), M, F, act, dgu.data_ptr(), _ptr(amax), _stream())
+    _count(1 if dh.numel() else 0)
+    return GatedGradResult(dgu if want_dgu else None, quantize_mxfp8(dgu) if quantize else None, amax)
 
 
 def set_launch_overlap(enabled: bool) -> bool:

@@ -16,6 +16,17 @@ mxfp8_output_t = torch.float8_e4m3fn
 mxfp8_scale_t = torch.uint8  # E8M0 byte = exponent + 127
 
 
+def as_quantize_result(r: kernels.Quantized) -> Q.QuantizeResult:
+    """A kernel's MXFP8 copies as the operator interface hands them on."""
+    r.scale._mt_swz = r.scale_swz
+    data_t = None
+    if r.data_t is not None:
+        r.scale_t._mt_swz = r.scale_t_swz
+        data_t = r.data_t.view(mxfp8_output_t)
+    return Q.QuantizeResult(r.data.view(mxfp8_output_t), r.scale, data_t, r.scale_t, None, None,
+                            r.scale_swz, r.scale_t_swz)
+
+
 class Mxfp8QuantizeOp(Q.QuantizeOpBase):
     format_name = "mxfp8"
 
@@ -26,14 +37,14 @@ class Mxfp8QuantizeOp(Q.QuantizeOpBase):
     def quantize(self, x, qparams, return_transpose=False, reduce_amax=False, tp_group=None, input_meta=None):
         assert qparams.quant_tile_shape in (None, (1, 32)), "MXFP8 uses 1x32 tiles"
         x = _as_2d_bf16(x)
-        r = kernels.quantize_mxfp8(x, return_transpose=return_transpose, into=getattr(input_meta, "into", None))
-        r.scale._mt_swz = r.scale_swz
-        data_t = None
-        if return_transpose:
-            r.scale_t._mt_swz = r.scale_t_swz
-            data_t = r.data_t.view(mxfp8_output_t)
-        return Q.QuantizeResult(r.data.view(mxfp8_output_t), r.scale, data_t, r.scale_t, None, None,
-                                r.scale_swz, r.scale_t_swz)
+        into = getattr(input_meta, "into", None)
+        made = getattr(input_meta, "quantized", None)
+        if made is not None and into is None and (made.data_t is not None or not return_transpose):
+            if tuple(made.data.shape) != tuple(x.shape):
+                raise kernels._lib.MtError(f"copies of a {tuple(made.data.shape)} tensor given for one of shape {tuple(x.shape)}")
+            return made
+        r = kernels.quantize_mxfp8(x, return_transpose=return_transpose, into=into)
+        return as_quantize_result(r)
 
     def sm_margin(self, sms: int):
         """Context in which this op's GEMMs leave `sms` SMs idle (for a collective in flight)."""
@@ -57,6 +68,19 @@ class Mxfp8QuantizeOp(Q.QuantizeOpBase):
         y = kernels.gemm_mxfp8(qx.view(torch.uint8), _swizzled(sx, M), qw.view(torch.uint8), _swizzled(sw, N),
                                out_dtype=kdt, out=out, accumulate=accumulate, bias=bias)
         return y if kdt == out_dtype or not isinstance(y, torch.Tensor) else y.to(out_dtype)
+
+    # ---- gated projection (GatedLinear) ----
+    def gated_qgemm(self, qx, qw, sx, sw, activation, global_amax_qx=None, global_amax_qw=None, want_h=True, want_gu=False,
+                    quantize_h=False, want_amax=False) -> kernels.GatedResult:
+        """act(x Wg^T) * (x Wu^T) with qw the quantized [Wg; Wu]."""
+        return kernels.gemm_gated_mxfp8(qx.view(torch.uint8), _swizzled(sx, qx.shape[0]), qw.view(torch.uint8),
+                                        _swizzled(sw, qw.shape[0]), activation=activation, sb_lin=sw.view(torch.uint8),
+                                        want_h=want_h, want_gu=want_gu, quantize_h=quantize_h, want_amax=want_amax)
+
+    def gated_backward(self, dh, gu, qparams, activation) -> Q.QuantizeResult:
+        """Quantized gradient [dg | du] (row-wise and transposed) of the two projections."""
+        assert qparams.quant_tile_shape in (None, (1, 32)), "MXFP8 uses 1x32 tiles"
+        return as_quantize_result(kernels.gated_backward(dh, gu, activation=activation).quantized)
 
     # ---- grouped (per-expert) operations used by GroupedLinear ----
     def grouped_quantize(self, w: torch.Tensor, qparams, return_transpose: bool = False) -> Q.QuantizeResult:

@@ -128,3 +128,18 @@ class Nvfp4TiledQuantizeOp(Q.QuantizeOpBase):
         y = kernels.gemm_nvfp4(qx, _swizzled(sx, M), global_amax_qx, qw, _swizzled(sw, N), global_amax_qw,
                                out_dtype=kdt, out=out, accumulate=accumulate, bias=bias)
         return y if kdt == out_dtype or not isinstance(y, torch.Tensor) else y.to(out_dtype)
+
+    # ---- gated projection (GatedLinear) ----
+    def gated_qgemm(self, qx, qw, sx, sw, activation, global_amax_qx=None, global_amax_qw=None, want_h=True, want_gu=False,
+                    quantize_h=False, want_amax=False) -> kernels.GatedResult:
+        """act(x Wg^T) * (x Wu^T) with qw the quantized [Wg; Wu]."""
+        assert global_amax_qx is not None and global_amax_qw is not None, "NVFP4 needs the per-tensor abs-max"
+        return kernels.gemm_gated_nvfp4(qx, _swizzled(sx, qx.shape[0]), global_amax_qx, qw, _swizzled(sw, qw.shape[0]),
+                                        global_amax_qw, activation=activation, sb_lin=sw.view(torch.uint8), want_h=want_h,
+                                        want_gu=want_gu, quantize_h=quantize_h, want_amax=want_amax)
+
+    def gated_backward(self, dh, gu, qparams, activation) -> Q.QuantizeResult:
+        """Quantized gradient [dg | du] (row-wise and transposed) of the two projections; its abs-max comes from
+        the kernel that computes it (the transformed copy still needs a pass of its own)."""
+        r = kernels.gated_backward(dh, gu, activation=activation, quantize=False, want_dgu=True, want_amax=not qparams.with_rht)
+        return self.quantize(r.dgu, qparams, return_transpose=True, input_meta=Q.QuantizeInputMeta(amax=r.amax))

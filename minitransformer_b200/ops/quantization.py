@@ -122,12 +122,16 @@ class QuantizeInputMeta(QuantizeInputMetaBase):
         place, used instead of the process-group all-reduce when reduce_amax is set.
     col_sum: fp32 [features] tensor that receives the column sums of the input from the
         quantizer's abs-max pass (the bias gradient, when the input is dy); the quantizer sets
-        col_sum_done when it has filled it (formats without an abs-max pass leave it alone)."""
+        col_sum_done when it has filled it (formats without an abs-max pass leave it alone).
+    quantized: the copies of exactly this tensor, made by its producer (RMSNorm or GatedLinear with
+        emit_quantized); the MXFP8 quantizer returns them instead of reading the tensor again,
+        where they hold what the call needs (the transposed copy too when that is asked for)."""
     amax_col: Optional[torch.Tensor] = None
     into: Optional[dict] = None
     amax_reduce: Optional[object] = None
     col_sum: Optional[torch.Tensor] = None
     col_sum_done: bool = False
+    quantized: Optional[QuantizeResult] = None
 
 
 class QuantizeOpBase:
