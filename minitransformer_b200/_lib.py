@@ -75,12 +75,12 @@ _SIGNATURES = {
                               _int, _vp]),
     "mt_peer_reduce_bf16": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
     "mt_rmsnorm_forward": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _c.c_float, _vp, _vp, _vp, _vp, _vp, _vp,
-                                  _i64, _vp, _vp]),
+                                  _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
     "mt_rmsnorm_backward_workspace": (_i64, [_i64, _i64]),
     "mt_rmsnorm_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "mt_gemm_gated_mxfp8": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _gated, _vp]),
     "mt_gemm_gated_nvfp4": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _gated, _vp]),
-    "mt_gated_backward": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp]),
+    "mt_gated_backward": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
     "mt_read_device_status": (_int, [_c.POINTER(_int), _vp]),
 }
 

@@ -7,7 +7,7 @@
 // in the rounding to bf16.
 #pragma once
 
-#include "mt_common.cuh"
+#include "quantize_common.cuh"
 
 namespace mt {
 
@@ -18,7 +18,19 @@ static inline bool gated_act_known(int act) { return act == MT_ACT_SILU || act =
 constexpr float GELU_C = 0.7978845608028654f;   // sqrt(2 / pi)
 constexpr float GELU_A = 0.044715f;
 
-__device__ __forceinline__ float gated_sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+// 1 / (1 + e^-z), e^-z = 2^(-z log2 e)
+__device__ __forceinline__ float gated_sigmoid(float z) { return rcp_approx(1.0f + ex2_approx(-LOG2E * z)); }
 
 template <int kAct>
 __device__ __forceinline__ float gated_act(float g) {
@@ -26,18 +38,24 @@ __device__ __forceinline__ float gated_act(float g) {
   return g * gated_sigmoid(2.0f * GELU_C * g * fmaf(GELU_A * g, g, 1.0f));
 }
 
-// act(g) and act'(g)
+// act(g) and act'(g) of two values at once
 template <int kAct>
-__device__ __forceinline__ void gated_act_grad(float g, float& act, float& grad) {
+__device__ __forceinline__ void gated_act_grad2(f32x2_t g, f32x2_t& act, f32x2_t& grad) {
+  const f32x2_t one = pack2(1.0f, 1.0f);
+  f32x2_t z, slope = g;
   if (kAct == MT_ACT_SILU) {
-    const float s = gated_sigmoid(g);
-    act = g * s;
-    grad = s * fmaf(g, 1.0f - s, 1.0f);
+    z = mul2(g, pack2(-LOG2E, -LOG2E));
   } else {
-    const float s = gated_sigmoid(2.0f * GELU_C * g * fmaf(GELU_A * g, g, 1.0f));
-    act = g * s;
-    grad = fmaf(act * (1.0f - s), 2.0f * GELU_C * fmaf(3.0f * GELU_A * g, g, 1.0f), s);
+    const f32x2_t gg = mul2(g, g);
+    z = mul2(mul2(g, pack2(-LOG2E * 2.0f * GELU_C, -LOG2E * 2.0f * GELU_C)), fma2(gg, pack2(GELU_A, GELU_A), one));
+    slope = mul2(mul2(g, pack2(2.0f * GELU_C, 2.0f * GELU_C)), fma2(gg, pack2(3.0f * GELU_A, 3.0f * GELU_A), one));
   }
+  float z0, z1, s0, s1;
+  unpack2(z, z0, z1);
+  unpack2(add2(pack2(ex2_approx(z0), ex2_approx(z1)), one), s0, s1);
+  const f32x2_t s = pack2(rcp_approx(s0), rcp_approx(s1));
+  act = mul2(g, s);
+  grad = mul2(s, fma2(slope, sub2(one, s), one));   // s + slope s (1 - s)
 }
 
 #endif  // __CUDACC__

@@ -9,7 +9,7 @@
 // Both directions move every element once and do a few operations on it: they are bound by HBM
 // (forward with residual and codes: 2 + 2 read, 2 + 1 written per element; backward 2 + 2 (+ 2)
 // read, 2 written).
-#include "quantize_common.cuh"
+#include "tile_quant.cuh"
 
 namespace mt {
 
@@ -26,9 +26,41 @@ struct RmsNormArgs {
   float* rstd;
   __nv_bfloat16* y;
   float* amax;
-  uint8_t *q, *s, *s_swz;
-  int64_t s_stride, kc;
+  int cluster;         // CTAs per panel (rmsnorm_panel_kernel)
+  MxTileOut out;
 };
+
+// Order in which both forward kernels add the squares of a row, so that a row's result does not
+// depend on which of them ran: eight columns in turn; the eight such sums of a 64-column segment by a
+// tree over lanes 4, 2, 1 apart; the eight segments of a 512-column group in turn; the groups in turn.
+__device__ __forceinline__ float sum_squares8(const uint4& w) {
+  float s = bf16_lo(w.x) * bf16_lo(w.x);
+  s = fmaf(bf16_hi(w.x), bf16_hi(w.x), s);
+  s = fmaf(bf16_lo(w.y), bf16_lo(w.y), s);
+  s = fmaf(bf16_hi(w.y), bf16_hi(w.y), s);
+  s = fmaf(bf16_lo(w.z), bf16_lo(w.z), s);
+  s = fmaf(bf16_hi(w.z), bf16_hi(w.z), s);
+  s = fmaf(bf16_lo(w.w), bf16_lo(w.w), s);
+  return fmaf(bf16_hi(w.w), bf16_hi(w.w), s);
+}
+__device__ __forceinline__ float rstd_of(float sum, int64_t cols, float eps) {
+  return __frsqrt_rn(__fdiv_rn(sum, (float)cols) + eps);
+}
+__device__ __forceinline__ uint4 add_bf16x8(const uint4& a, const uint4& b) {
+  uint4 o;
+  o.x = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.x), bf16x2_to_f32x2(b.x)));
+  o.y = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.y), bf16x2_to_f32x2(b.y)));
+  o.z = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.z), bf16x2_to_f32x2(b.z)));
+  o.w = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.w), bf16x2_to_f32x2(b.w)));
+  return o;
+}
+__device__ __forceinline__ void scale_row8(const uint4& w, float rstd, const float (&g)[8], uint32_t (&y)[4]) {
+  const f32x2_t r2 = pack2(rstd, rstd);
+  y[0] = f32x2_to_bf16x2(mul2(mul2(bf16x2_to_f32x2(w.x), r2), pack2(g[0], g[1])));
+  y[1] = f32x2_to_bf16x2(mul2(mul2(bf16x2_to_f32x2(w.y), r2), pack2(g[2], g[3])));
+  y[2] = f32x2_to_bf16x2(mul2(mul2(bf16x2_to_f32x2(w.z), r2), pack2(g[4], g[5])));
+  y[3] = f32x2_to_bf16x2(mul2(mul2(bf16x2_to_f32x2(w.w), r2), pack2(g[6], g[7])));
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -58,47 +90,51 @@ __device__ __forceinline__ void load_gamma8(const void* gamma, int is_f32, int64
   }
 }
 
-// One CTA per row, V vectors of 8 columns per thread (vector i * blockDim + thread). The row stays
-// in registers between the sum and the scaling. A 1x32 block is four adjacent lanes. CTAs
-// beyond the last row fill the padding of the GEMM-layout scales with zeros.
+// Rows without a transposed copy. One CTA per row, V vectors of 8 columns per thread (vector
+// i * blockDim + thread). The row stays in registers between the sum and the scaling. A 1x32 block is
+// four adjacent lanes. CTAs beyond the last row fill the padding of the GEMM-layout scales with zeros.
 template <int V>
 __global__ void __launch_bounds__(1024) rmsnorm_rows_kernel(const RmsNormArgs a) {
-  __shared__ float slot[32];
+  __shared__ float4 seg4[RN_MAX_COLS / 256];   // sums of 64-column segments, a group being two of these
+  float* seg = reinterpret_cast<float*>(seg4);
+  const MxTileOut& o = a.out;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
   pdl_trigger();
   pdl_wait();
   if (row >= a.rows) {
-    uint8_t* cell = a.s_swz + (row >> 7) * a.kc * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
-    for (int64_t c = tid; c < a.kc; c += blockDim.x) *reinterpret_cast<uint32_t*>(cell + c * 512) = 0u;
+    uint8_t* cell = o.s_swz + (row >> 7) * o.kc_row * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+    for (int64_t c = tid; c < o.kc_row; c += blockDim.x) *reinterpret_cast<uint32_t*>(cell + c * 512) = 0u;
     return;
   }
   uint4 w[V];
-  float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = i * blockDim.x + tid;
     w[i] = make_uint4(0, 0, 0, 0);
     if (v < nvec) {
       w[i] = *reinterpret_cast<const uint4*>(a.x + row * a.x_stride + (int64_t)v * 8);
-      if (a.r != nullptr) {
-        const uint4 r = *reinterpret_cast<const uint4*>(a.r + row * a.r_stride + (int64_t)v * 8);
-        w[i].x = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].x), bf16x2_to_f32x2(r.x)));
-        w[i].y = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].y), bf16x2_to_f32x2(r.y)));
-        w[i].z = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].z), bf16x2_to_f32x2(r.z)));
-        w[i].w = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(w[i].w), bf16x2_to_f32x2(r.w)));
-        if (a.h != nullptr) *reinterpret_cast<uint4*>(a.h + row * a.cols + (int64_t)v * 8) = w[i];
-      }
-    }
-    const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      ss = fmaf(bf16_lo(ws[j]), bf16_lo(ws[j]), ss);
-      ss = fmaf(bf16_hi(ws[j]), bf16_hi(ws[j]), ss);
+      if (a.r != nullptr) w[i] = add_bf16x8(w[i], *reinterpret_cast<const uint4*>(a.r + row * a.r_stride + (int64_t)v * 8));
     }
   }
-  ss = block_sum(ss, slot);
-  const float rstd = __frsqrt_rn(__fdiv_rn(ss, (float)a.cols) + a.eps);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    if (a.h != nullptr && v < nvec) *reinterpret_cast<uint4*>(a.h + row * a.cols + (int64_t)v * 8) = w[i];
+    float ss = sum_squares8(w[i]);
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    if ((tid & 7) == 0) seg[v >> 3] = ss;      // (V * blockDim) / 8 segments, zeros beyond the row
+  }
+  __syncthreads();
+  const int groups = (int)(V * blockDim.x) >> 6;   // blockDim is a multiple of 64
+  float total = 0.0f;
+#pragma unroll 4
+  for (int j = 0; j < groups; ++j) {
+    const float4 p = seg4[2 * j], u = seg4[2 * j + 1];
+    total += ((((((p.x + p.y) + p.z) + p.w) + u.x) + u.y) + u.z) + u.w;
+  }
+  const float rstd = rstd_of(total, a.cols, a.eps);
   if (tid == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
 
   uint32_t am = 0;
@@ -110,41 +146,205 @@ __global__ void __launch_bounds__(1024) rmsnorm_rows_kernel(const RmsNormArgs a)
     uint32_t yw[4] = {0, 0, 0, 0};
     if (on) {
       load_gamma8(a.gamma, a.gamma_f32, (int64_t)v * 8, g);
-      const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-      const f32x2_t r2 = pack2(rstd, rstd);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        yw[j] = f32x2_to_bf16x2(mul2(mul2(bf16x2_to_f32x2(ws[j]), r2), pack2(g[2 * j], g[2 * j + 1])));
+      scale_row8(w[i], rstd, g, yw);
       if (a.y != nullptr)
         *reinterpret_cast<uint4*>(a.y + row * a.cols + (int64_t)v * 8) = make_uint4(yw[0], yw[1], yw[2], yw[3]);
     }
     uint32_t m = absmax2(absmax2(yw[0], yw[1]), absmax2(yw[2], yw[3]));
     am = absmax2(am, m);
-    if (a.q != nullptr) {
+    if (o.q != nullptr) {
       m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const int e = e8m0_exponent(absmax2_to_float(m));
+      uint32_t f;
+      const uint8_t sb = static_cast<uint8_t>(mx_scale(mx_amax_bits(m), f));
       if (on) {
-        const float enc = exp2_neg(e);
+        const float enc = __uint_as_float(f << 16);
         const f32x2_t enc2 = pack2(enc, enc);
-        *reinterpret_cast<uint2*>(a.q + row * a.cols + (int64_t)v * 8) =
+        *reinterpret_cast<uint2*>(o.q + row * a.cols + (int64_t)v * 8) =
             make_uint2(e4m3x4_from_words(yw[0], yw[1], enc2), e4m3x4_from_words(yw[2], yw[3], enc2));
         if ((v & 3) == 0) {
           const int kb = v >> 2;
-          a.s[row * a.s_stride + kb] = static_cast<uint8_t>(e + 127);
-          if (a.s_swz != nullptr)
-            a.s_swz[((row >> 7) * a.kc + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), kb)] = static_cast<uint8_t>(e + 127);
+          o.s[row * o.s_stride + kb] = sb;
+          if (o.s_swz != nullptr)
+            o.s_swz[((row >> 7) * o.kc_row + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), kb)] = sb;
         }
       }
     }
   }
-  if (a.s_swz != nullptr)   // blocks beyond the row, up to the padded chunk count
-    for (int64_t kb = (a.cols >> 5) + tid; kb < a.kc * 4; kb += blockDim.x)
-      a.s_swz[((row >> 7) * a.kc + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)kb)] = 0;
+  if (o.s_swz != nullptr)   // blocks beyond the row, up to the padded chunk count
+    for (int64_t kb = (a.cols >> 5) + tid; kb < o.kc_row * 4; kb += blockDim.x)
+      o.s_swz[((row >> 7) * o.kc_row + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)kb)] = 0;
   if (a.amax != nullptr) {
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
     if ((tid & 31) == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
   }
+}
+
+// With a transposed copy. A cluster of C CTAs owns a panel of 32 rows, each CTA 64 columns per warp of
+// it, each warp one 32 x 64 tile in registers (layout of tile_quant.cuh). x is read once: the sums of
+// squares of 512-column groups go to every CTA of the cluster through distributed shared memory,
+// then the tiles are scaled and quantized both ways in place. 32 words of data per thread leave
+// room for 32 warps per SM, enough that some CTAs load while others wait for their cluster or store.
+// Panels beyond the last row (up to 128 rows) and the last panel write the scales' padding.
+constexpr int RN_PANEL_MAX_COLS = 16384;
+
+template <int kMaxThreads, int kMinCtas>
+__global__ void __launch_bounds__(kMaxThreads, kMinCtas) rmsnorm_panel_kernel(const RmsNormArgs a) {
+  constexpr int WARPS = kMaxThreads / 32;
+  __shared__ float seg[WARPS][32];                      // this CTA's segments
+  __shared__ float grp[RN_PANEL_MAX_COLS / 512][32];    // the panel's groups
+  __shared__ __align__(16) uint8_t s_row[32][WARPS * 2];
+  const MxTileOut& o = a.out;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int cg = lane & 7, rg = lane >> 3;
+  const int rank = (int)cluster_ctarank(), ranks = a.cluster;
+  const int64_t panel = blockIdx.x / ranks, row0 = panel * 32;
+  const int64_t cta_col0 = (int64_t)rank * warps * 64, col0 = cta_col0 + warp * 64;
+  const int64_t r0 = row0 + rg * 8, c = col0 + cg * 8;
+  const bool c_ok = c < a.cols;
+  pdl_trigger();
+  pdl_wait();
+  uint4 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (c_ok && r0 + i < a.rows) w[i] = *reinterpret_cast<const uint4*>(a.x + (r0 + i) * a.x_stride + c);
+  }
+  if (a.r != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c_ok && r0 + i < a.rows) {
+        w[i] = add_bf16x8(w[i], *reinterpret_cast<const uint4*>(a.r + (r0 + i) * a.r_stride + c));
+        *reinterpret_cast<uint4*>(a.h + (r0 + i) * a.cols + c) = w[i];
+      }
+  }
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = sum_squares8(w[i]);
+  // eight row sums over eight lanes: every exchange halves the rows a lane still carries
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float send = (cg & 4) ? v[i] : v[i + 4], keep = (cg & 4) ? v[i + 4] : v[i];
+    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float send = (cg & 2) ? v[i] : v[i + 2], keep = (cg & 2) ? v[i + 2] : v[i];
+    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2);
+  }
+  {
+    const float send = (cg & 1) ? v[0] : v[1], keep = (cg & 1) ? v[1] : v[0];
+    v[0] = keep + __shfl_xor_sync(0xffffffffu, send, 1);
+  }
+  seg[warp][lane] = v[0];       // lane l: row l of the panel
+  if (ranks > 1) cluster_arrive();
+  __syncthreads();
+  if (ranks > 1) cluster_wait();   // every CTA of the cluster has started before anything is written into it
+  const int groups = (warps + 7) >> 3;
+  if (warp < groups) {
+    float sum = seg[warp * 8][lane];
+#pragma unroll
+    for (int j = 1; j < 8; ++j)
+      if (warp * 8 + j < warps) sum += seg[warp * 8 + j][lane];
+    const uint32_t mine = smem_u32(&grp[rank * groups + warp][lane]);
+    if (ranks == 1) grp[warp][lane] = sum;
+    else
+      for (int r = 0; r < ranks; ++r)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(mine, (uint32_t)r)), "f"(sum) : "memory");
+  }
+  if (ranks > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  float total = 0.0f;
+#pragma unroll 4
+  for (int j = 0; j < ranks * groups; ++j) total += grp[j][lane];
+  const float rstd_l = rstd_of(total, a.cols, a.eps);
+  if (rank == 0 && warp == 0 && a.rstd != nullptr && row0 + lane < a.rows) a.rstd[row0 + lane] = rstd_l;
+  if (col0 < a.cols) {          // uniform for the warp
+    float g[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g[k] = 0.0f;
+    if (c_ok) load_gamma8(a.gamma, a.gamma_f32, c, g);
+    uint32_t yw[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float rs = __shfl_sync(0xffffffffu, rstd_l, rg * 8 + i);
+      if (r0 + i < a.rows) scale_row8(w[i], rs, g, yw[i]);
+      else yw[i][0] = yw[i][1] = yw[i][2] = yw[i][3] = 0;
+      if (a.y != nullptr && c_ok && r0 + i < a.rows)
+        *reinterpret_cast<uint4*>(a.y + (r0 + i) * a.cols + c) = make_uint4(yw[i][0], yw[i][1], yw[i][2], yw[i][3]);
+    }
+    if (a.amax != nullptr) {
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) am = absmax2(am, absmax2(absmax2(yw[i][0], yw[i][1]), absmax2(yw[i][2], yw[i][3])));
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
+      if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
+    }
+    const MxTileScales sc = mx_tile_store(o, yw, row0, col0, a.cols);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      s_row[rg * 8 + (lane & 3) * 2 + j][warp * 2 + (cg >> 2)] = static_cast<uint8_t>(sc.row[j]);
+      const int64_t f = col0 + cg * 8 + rg * 2 + j;
+      if (f < a.cols) {
+        if (row0 < o.rows) o.s_t[f * o.s_t_stride + panel] = static_cast<uint8_t>(sc.col[j]);
+        if (o.s_t_swz != nullptr)
+          o.s_t_swz[((f >> 7) * o.kc_col + (panel >> 2)) * 512 + sf_chunk_offset((int)(f & 127), (int)(panel & 3))] =
+              static_cast<uint8_t>(sc.col[j]);
+      }
+    }
+  }
+  __syncthreads();
+  {
+    // row scales: a word (four blocks) per row and pair of warps
+    const int64_t r = row0 + lane, b0 = (cta_col0 >> 5) + warp * 4, nb = a.cols >> 5;
+    if (warp * 2 < warps && b0 < nb) {
+      const int n = (int)min((int64_t)min(4, warps * 2 - warp * 4), nb - b0);
+      uint32_t word = 0;
+      for (int i = 0; i < n; ++i) word |= static_cast<uint32_t>(s_row[lane][warp * 4 + i]) << (8 * i);
+      mx_store_scale_word(word, n, r < o.rows ? o.s + r * o.s_stride + b0 : nullptr, o.s_swz, r, b0, o.kc_row);
+    }
+  }
+  const bool last_rank = rank == ranks - 1;
+  if (last_rank) {
+    mx_pad_row_scales(o, row0, 32, tid, blockDim.x);
+    mx_pad_col_features(o, panel, tid, blockDim.x);
+  }
+  if (panel == gridDim.x / ranks - 1) {
+    const int64_t c0 = min(cta_col0, a.cols), c1 = min(c0 + (int64_t)warps * 64, a.cols);
+    if (c1 > c0) mx_pad_col_blocks(o, panel + 1, c0, c1, tid, blockDim.x);
+    if (last_rank) mx_pad_col_blocks(o, panel + 1, a.cols, (a.cols + 127) / 128 * 128, tid, blockDim.x);
+  }
+}
+
+// 512 columns (8 warps) per CTA and up to 8 CTAs per panel; longer rows take 16 or 32 warps per CTA. Groups of 512
+// columns never straddle two CTAs.
+static int launch_rmsnorm_panel(RmsNormArgs& a, cudaStream_t st) {
+  int warps = 8, ranks = (int)((a.cols + 511) / 512);
+  if (a.cols <= 512) warps = (int)((a.cols + 63) / 64);
+  while (ranks > 8) {
+    warps *= 2;
+    ranks = (int)((a.cols + 64 * warps - 1) / (64 * warps));
+  }
+  a.cluster = ranks;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.rows + 127) / 128 * 4 * ranks));
+  cfg.blockDim = dim3(32 * warps);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const RmsNormArgs& ca = a;
+  if (warps <= 8) MT_CUDA(cudaLaunchKernelEx(&cfg, rmsnorm_panel_kernel<256, 4>, ca));
+  else MT_CUDA(cudaLaunchKernelEx(&cfg, rmsnorm_panel_kernel<1024, 1>, ca));
+  return MT_OK;
 }
 
 // ---- gradient ----
@@ -269,8 +469,8 @@ static int rn_sm_count() {
   return n[slot];
 }
 
-// Threads per row for V vectors per thread.
-static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / V + 31) / 32 * 32); }
+// Threads per row for V vectors per thread (a multiple of 64: whole groups of four segments).
+static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / V + 63) / 64 * 64); }
 
 static int rn_grad_ctas(int64_t rows) {
   const int64_t most = 2 * (int64_t)rn_sm_count();
@@ -283,15 +483,15 @@ static bool row_aligned(const void* p, int64_t stride) { return aligned16(p) && 
 
 extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* residual, int64_t r_stride, const void* gamma,
                                   int gamma_dtype, int64_t rows, int64_t cols, float eps, void* h, float* rstd, void* y,
-                                  float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz,
-                                  mt_stream_t stream) {
+                                  float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz, uint8_t* q_t,
+                                  uint8_t* s_t, int64_t s_t_stride, uint8_t* s_t_swz, mt_stream_t stream) {
   using namespace mt;
   const char* name = "mt_rmsnorm_forward";
   MT_REQUIRE(rows >= 0 && cols > 0 && cols <= RN_MAX_COLS, "%s: cols (%lld) must be within [1, %d]", name, (long long)cols, RN_MAX_COLS);
   MT_REQUIRE(cols % 8 == 0, "%s: cols (%lld) must be a multiple of 8", name, (long long)cols);
   MT_REQUIRE(gamma_dtype == MT_BF16 || gamma_dtype == MT_F32, "%s: gamma dtype %d not supported", name, gamma_dtype);
   MT_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", name);
-  MT_REQUIRE(rows < (int64_t)1 << 31, "%s: too many rows", name);
+  MT_REQUIRE(rows < (int64_t)1 << 30, "%s: too many rows", name);
   if (rows == 0) return MT_OK;
   MT_REQUIRE(x && gamma, "%s: null x / gamma", name);
   MT_REQUIRE(x_stride >= cols && row_aligned(x, x_stride), "%s: x needs 16-byte aligned rows", name);
@@ -299,23 +499,22 @@ extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* r
   MT_REQUIRE(!residual || h, "%s: a residual needs an output for the sum", name);
   MT_REQUIRE(residual || !h, "%s: without a residual there is no sum to write", name);
   MT_REQUIRE(aligned16(gamma) && aligned16(h) && aligned16(y), "%s: pointers must be 16-byte aligned", name);
-  if (q) {
-    MT_REQUIRE(cols % 32 == 0, "%s: cols (%lld) must be a multiple of 32 for the MXFP8 copy", name, (long long)cols);
-    MT_REQUIRE(s && s_stride >= cols / 32, "%s: the MXFP8 copy needs s with a stride of at least cols / 32", name);
-    MT_REQUIRE(aligned16(q) && aligned16(s_swz), "%s: q and s_swz must be 16-byte aligned", name);
-  } else {
-    MT_REQUIRE(!s && !s_swz, "%s: scales without codes", name);
-  }
+  int rc = mx_outputs_ok(name, rows, cols, q, s, s_stride, s_swz, q_t, s_t, s_t_stride, s_t_swz);
+  if (rc != MT_OK) return rc;
+  if (q_t && cols > RN_PANEL_MAX_COLS)
+    return fail(MT_ERR_UNSUPPORTED, "%s: a transposed copy of more than %d columns: quantize y instead", name, RN_PANEL_MAX_COLS);
   RmsNormArgs a{};
   a.x = static_cast<const __nv_bfloat16*>(x); a.x_stride = x_stride;
   a.r = static_cast<const __nv_bfloat16*>(residual); a.r_stride = r_stride;
   a.gamma = gamma; a.gamma_f32 = gamma_dtype == MT_F32;
   a.rows = rows; a.cols = cols; a.eps = eps;
   a.h = static_cast<__nv_bfloat16*>(h); a.rstd = rstd; a.y = static_cast<__nv_bfloat16*>(y); a.amax = amax;
-  a.q = q; a.s = s; a.s_swz = s_swz; a.s_stride = s_stride;
-  a.kc = ((cols / 32 + 3) / 4 + 3) / 4 * 4;
+  a.out = {q, s, s_swz, q_t, s_t, s_t_swz, rows, cols, s_stride, s_t_stride, mx_padded_chunks(cols / 32),
+           mx_padded_chunks((rows + 31) / 32)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)(s_swz ? (rows + 127) / 128 * 128 : rows));
+  const int64_t padded = (rows + 127) / 128 * 128;
+  if (q_t) return launch_rmsnorm_panel(a, st);
+  const dim3 grid((unsigned)(s_swz ? padded : rows));
   if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<1>, grid, dim3(rn_threads(cols, 1)), 0, st, a));
   else if (cols <= 16384) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<2>, grid, dim3(rn_threads(cols, 2)), 0, st, a));
   else MT_CUDA(launch_pdl(rmsnorm_rows_kernel<4>, grid, dim3(rn_threads(cols, 4)), 0, st, a));

@@ -562,6 +562,23 @@ def _amax_scalar(device) -> torch.Tensor:
     return torch.zeros(1, dtype=torch.float32, device=device) if z is None else z
 
 
+def _mxfp8_outputs(rows: int, cols: int, transpose: bool, device) -> Quantized:
+    """Buffers for the MXFP8 copies of a [rows, cols] tensor."""
+    u8 = torch.uint8
+    c = Quantized(torch.empty((rows, cols), dtype=u8, device=device), torch.empty((rows, cols // 32), dtype=u8, device=device),
+                  torch.empty(swizzled_scale_bytes(rows, cols // 32), dtype=u8, device=device))
+    if transpose:
+        mb = (rows + 31) // 32
+        c.data_t = torch.empty((cols, rows), dtype=u8, device=device)
+        c.scale_t = torch.empty((cols, mb), dtype=u8, device=device)
+        c.scale_t_swz = torch.empty(swizzled_scale_bytes(cols, mb), dtype=u8, device=device)
+    return c
+
+
+_NO_COPIES = Quantized(None, None, None)
+_NORM_PANEL_COLS = 16384     # columns up to which mt_rmsnorm_forward makes a transposed copy
+
+
 @dataclass
 class RmsNormResult:
     """h: x + residual in bf16 (x itself without a residual); rstd fp32 [rows]; y bf16 or None; quantized:
@@ -588,27 +605,22 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residua
     weight = _gamma(weight, C)
     if not (want_y or quantize):
         raise _lib.MtError("rmsnorm: neither y nor its MXFP8 copies requested")
-    dev, u8 = x.device, torch.uint8
-    return_transpose = return_transpose and quantize
+    dev = x.device
     h = x if residual is None else torch.empty((M, C), dtype=torch.bfloat16, device=dev)
     rstd = torch.empty(M, dtype=torch.float32, device=dev)
-    y = torch.empty((M, C), dtype=torch.bfloat16, device=dev) if want_y or return_transpose else None
+    # rows too long for the kernel that makes both copies: y, then the quantize kernel
+    after = quantize and return_transpose and C > _NORM_PANEL_COLS
+    y = torch.empty((M, C), dtype=torch.bfloat16, device=dev) if want_y or after else None
     amax = _amax_scalar(dev) if want_amax else None
-    q = s = s_swz = None
-    if quantize and not return_transpose:
-        q = torch.empty((M, C), dtype=u8, device=dev)
-        s = torch.empty((M, C // 32), dtype=u8, device=dev)
-        s_swz = torch.empty(swizzled_scale_bytes(M, C // 32), dtype=u8, device=dev)
+    c = _mxfp8_outputs(M, C, return_transpose, dev) if quantize and not after else _NO_COPIES
     _lib.call("mt_rmsnorm_forward", x.data_ptr(), _row_stride(x), _ptr(residual), 0 if residual is None else _row_stride(residual),
               weight.data_ptr(), _out_dtype_code(weight.dtype), M, C, eps, None if residual is None else h.data_ptr(),
-              rstd.data_ptr(), _ptr(y), _ptr(amax), _ptr(q), _ptr(s), C // 32, _ptr(s_swz), _stream())
+              rstd.data_ptr(), _ptr(y), _ptr(amax), _ptr(c.data), _ptr(c.scale), C // 32, _ptr(c.scale_swz), _ptr(c.data_t),
+              _ptr(c.scale_t), (M + 31) // 32, _ptr(c.scale_t_swz), _stream())
     _count(1 if M else 0)
-    quantized = None
-    if return_transpose:
-        quantized = quantize_mxfp8(y, return_transpose=True)
-    elif quantize:
-        quantized = Quantized(q, s, s_swz)
-    return RmsNormResult(h, rstd, y if want_y else None, quantized, amax)
+    if after:
+        c = quantize_mxfp8(y, return_transpose=True)
+    return RmsNormResult(h, rstd, y if want_y else None, c if quantize else None, amax)
 
 
 @_on_tensor_device
@@ -744,10 +756,13 @@ def gated_backward(dh: torch.Tensor, gu: torch.Tensor, *, activation: str = "sil
     if not (quantize or want_dgu):
         raise _lib.MtError("gated_backward: neither the gradient nor its MXFP8 copies requested")
     amax = _amax_scalar(dh.device) if want_amax else None
-    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dh.device)
-    _lib.call("mt_gated_backward", dh.data_ptr(), _row_stride(dh), gu.data_ptr(), M, F, act, dgu.data_ptr(), _ptr(amax), _stream())
+    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dh.device) if want_dgu else None
+    c = _mxfp8_outputs(M, 2 * F, True, dh.device) if quantize else _NO_COPIES
+    _lib.call("mt_gated_backward", dh.data_ptr(), _row_stride(dh), gu.data_ptr(), M, F, act, _ptr(dgu), _ptr(amax), _ptr(c.data),
+              _ptr(c.scale), 2 * F // 32, _ptr(c.scale_swz), _ptr(c.data_t), _ptr(c.scale_t), (M + 31) // 32, _ptr(c.scale_t_swz),
+              _stream())
     _count(1 if dh.numel() else 0)
-    return GatedGradResult(dgu if want_dgu else None, quantize_mxfp8(dgu) if quantize else None, amax)
+    return GatedGradResult(dgu, c if quantize else None, amax)
 
 
 def set_launch_overlap(enabled: bool) -> bool:

@@ -26,8 +26,9 @@ def _refused(rc, text):
 def test_norm_entry_points_refuse(p):
     lib = _lib.load()
 
-    def fwd(x=p, xs=64, r=None, rs=0, g=p, gd=0, rows=2, cols=64, eps=1e-5, h=None, y=p, q=None, s=None, ss=2, swz=None):
-        return lib.mt_rmsnorm_forward(x, xs, r, rs, g, gd, rows, cols, eps, h, p, y, None, q, s, ss, swz, None)
+    def fwd(x=p, xs=64, r=None, rs=0, g=p, gd=0, rows=2, cols=64, eps=1e-5, h=None, y=p, q=None, s=None, ss=2, swz=None,
+            qt=None, st=None, sts=1):
+        return lib.mt_rmsnorm_forward(x, xs, r, rs, g, gd, rows, cols, eps, h, p, y, None, q, s, ss, swz, qt, st, sts, None, None)
 
     _refused(fwd(cols=12, xs=16), "multiple of 8")
     _refused(fwd(cols=0), "within")
@@ -45,8 +46,13 @@ def test_norm_entry_points_refuse(p):
     _refused(fwd(h=p), "no sum")
     _refused(fwd(y=p + 4), "16-byte")
     _refused(fwd(cols=40, xs=40, q=p, s=p), "multiple of 32")
-    _refused(fwd(q=p), "needs s")
-    _refused(fwd(q=p, s=p, ss=1), "needs s")
+    _refused(fwd(q=p), "need s")
+    _refused(fwd(q=p, s=p, ss=1), "need s")
+    _refused(fwd(q=p, s=p, qt=p), "need s_t")
+    _refused(fwd(q=p, s=p, qt=p, st=p, sts=0), "need s_t")
+    _refused(fwd(q=p, s=p, st=p), "without transposed codes")
+    _refused(fwd(qt=p, st=p), "without codes")
+    assert fwd(cols=16416, xs=16416, q=p, s=p, ss=513, qt=p, st=p) == -2
     _refused(fwd(q=p + 8, s=p), "16-byte")
     _refused(fwd(s=p), "without codes")
     assert fwd(rows=0, x=None) == 0                 # nothing to do
@@ -98,8 +104,18 @@ def test_gated_entry_points_refuse(p):
     rc = lib.mt_gemm_gated_nvfp4(p, p, None, p, p, None, p, 2, 128, 64, 0, out(h=p), None)
     _refused(rc, "abs-max")
 
-    def gb(dh=p, ds=64, gu=p, rows=2, F=64, act=0, dgu=p):
-        return lib.mt_gated_backward(dh, ds, gu, rows, F, act, dgu, None, None)
+    def gb(dh=p, ds=64, gu=p, rows=2, F=64, act=0, dgu=p, q=None, s=None, ss=4, qt=None, st=None, sts=1):
+        return lib.mt_gated_backward(dh, ds, gu, rows, F, act, dgu, None, q, s, ss, None, qt, st, sts, None, None)
+
+    _refused(gb(dgu=None), "no output")
+    _refused(gb(q=p), "codes need s")
+    _refused(gb(q=p, s=p, ss=3), "codes need s")
+    _refused(gb(q=p, s=p, qt=p), "need s_t")
+    _refused(gb(q=p, s=p, qt=p, st=p, sts=0), "need s_t")
+    _refused(gb(q=p, s=p, st=p), "without transposed codes")
+    _refused(gb(qt=p, st=p), "without codes")
+    _refused(gb(q=p + 8, s=p), "16-byte")
+    _refused(gb(rows=1 << 23), "out of range")
 
     _refused(gb(F=40), "multiple of 32")
     _refused(gb(act=5), "activation")
