@@ -362,7 +362,7 @@ int mt_peer_reduce_bf16(const void* stage, int n, int64_t rows, int64_t cols, vo
  * (gamma_dtype). Outputs, each optional (h required with a residual), rows contiguous:
  *   h bf16; rstd fp32 [rows]; y bf16; amax device fp32 scalar, raised to max |y| (zeroed by the caller);
  *   q, s (stride s_stride), s_swz, q_t, s_t (stride s_t_stride), s_t_swz: MXFP8 copies of y as
- *   mt_quantize_mxfp8 makes them (cols % 32 == 0; with q_t at most 16384 columns, beyond that
+ *   mt_quantize_mxfp8 makes them (cols % 32 == 0; with q_t at most 8192 columns, beyond that
  *   MT_ERR_UNSUPPORTED).
  * h may be the same buffer as x or residual. */
 int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
@@ -413,7 +413,7 @@ int mt_gemm_gated_nvfp4(const uint8_t* x, const uint8_t* sx_swz, const float* am
  * dh bf16 [rows, F] (row stride dh_stride), gu bf16 [rows, 2F] = [g | u]; F % 32 == 0.
  * Outputs, dgu or q at least: dgu bf16 [rows, 2F] = [dg | du]; amax (optional): device fp32 scalar, raised
  * to max |dgu| (zeroed by the caller); q, s, s_swz, q_t, s_t, s_t_swz: MXFP8 copies of dgu as
- * mt_quantize_mxfp8 makes them (q_t optional). rows < 2^23. */
+ * mt_quantize_mxfp8 makes them (q_t optional). */
 int mt_gated_backward(const void* dh, int64_t dh_stride, const void* gu, int64_t rows, int64_t F, int activation,
                       void* dgu, float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz,
                       uint8_t* q_t, uint8_t* s_t, int64_t s_t_stride, uint8_t* s_t_swz, mt_stream_t stream);

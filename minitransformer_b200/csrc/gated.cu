@@ -8,45 +8,62 @@
 namespace mt {
 
 struct GatedGradArgs {
-  const __nv_bfloat16 *dh, *gu;
-  int64_t dh_stride, rows, F;
+  int64_t rows, F;
+  int tiles_x, tiles;
+  int* status;
   __nv_bfloat16* dgu;
   float* amax;
   MxTileOut out;       // out.q null: no copies
 };
 
-// A CTA covers 128 rows x 128 features: four warps of 32 rows side by side in each of two 64-column halves, so that
-// row-wise codes leave in whole 128-byte lines and transposed codes in 128-byte runs of one feature. All loads of
-// a thread (24 of 16 bytes) are issued before the first is used: the two CTAs of an SM then keep 196 KB in flight,
-// and one computes while the other waits. Scale bytes are collected in shared memory and leave as words.
+// Persistent CTAs, two per SM; a CTA takes 128 rows x 128 features at a time: four warps of 32 rows side by side in
+// each of two 64-column halves, so that row-wise codes leave in whole 128-byte lines and transposed codes in
+// 128-byte runs of one feature. Every warp fetches its own 32 x 64 tiles of dh, g and u by TMA (12 KB, one
+// mbarrier per warp) and asks for the next ones as soon as it has computed dg and du into registers: they arrive
+// while the warp quantizes and stores. Scale bytes are collected in shared memory and leave as words.
+constexpr int GG_SMEM = 8 * 3 * MX_TILE_BYTES + 128;
+
 template <int kAct>
-__global__ void __launch_bounds__(256, 2) gated_grad_kernel(const GatedGradArgs a) {
+__global__ void __launch_bounds__(256, 2)
+    gated_grad_kernel(const __grid_constant__ CUtensorMap map_dh, const __grid_constant__ CUtensorMap map_gu, const GatedGradArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
   __shared__ __align__(16) uint8_t s_row[2][128][4], s_col[2][128][4];   // [dg, du][row / feature][block]
+  __shared__ uint64_t bars[8];
+  __shared__ int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t m0 = (int64_t)blockIdx.y * 128, f0 = (int64_t)blockIdx.x * 128;
   const int wr = warp & 3, wc = warp >> 2;
-  const int64_t row0 = m0 + wr * 32, c0 = f0 + wc * 64;
-  const int64_t row = row0 + (lane >> 3) * 8, f = c0 + (lane & 7) * 8;
-  const bool f_ok = f < a.F;
+  uint8_t* buf = smem + warp * 3 * MX_TILE_BYTES;
+  const MxTileOut& o = a.out;
+  const bool row_words = mx_word_aligned(o.s, o.s_stride), col_words = mx_word_aligned(o.s_t, o.s_t_stride);
+  if (tid == 0) abort_flag = 0;
+  if (lane == 0) mbar_init(&bars[warp], 1);
+  mbar_fence_init();
+  __syncthreads();
   pdl_trigger();
   pdl_wait();
-  uint4 d4[8], g4[8], u4[8];
-  const __nv_bfloat16* pd = a.dh + row * a.dh_stride + f;
-  const __nv_bfloat16* pg = a.gu + row * 2 * a.F + f;
+
+  auto fetch = [&](int tile) {
+    const int y = tile / a.tiles_x, x = tile - y * a.tiles_x;
+    const int32_t r = y * 128 + wr * 32, c = x * 128 + wc * 64;
+    mbar_expect_tx(&bars[warp], 3 * MX_TILE_BYTES);
+    tma_load_2d(buf, &map_gu, &bars[warp], c, r);
+    tma_load_2d(buf + MX_TILE_BYTES, &map_dh, &bars[warp], c, r);
+    tma_load_2d(buf + 2 * MX_TILE_BYTES, &map_gu, &bars[warp], (int32_t)a.F + c, r);
+  };
+  if (lane == 0 && (int)blockIdx.x < a.tiles) fetch(blockIdx.x);
+  uint32_t ph = 0;
+  for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ph ^= 1) {
+  const int ty = tile / a.tiles_x, tx = tile - ty * a.tiles_x;
+  const int64_t m0 = (int64_t)ty * 128, f0 = (int64_t)tx * 128;
+  const int64_t row0 = m0 + wr * 32, c0 = f0 + wc * 64;
+  // on expiry the status word tells; the warp goes on with what is there, so that nobody waits for it
+  mbar_wait_bounded(&bars[warp], ph, &abort_flag, a.status, DS_QUANT_WAIT);
+  uint32_t wg[8][4], wu[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    d4[i] = g4[i] = u4[i] = make_uint4(0, 0, 0, 0);
-    if (f_ok && row + i < a.rows) {
-      g4[i] = *reinterpret_cast<const uint4*>(pg + i * 2 * a.F);
-      d4[i] = *reinterpret_cast<const uint4*>(pd + i * a.dh_stride);
-      u4[i] = *reinterpret_cast<const uint4*>(pg + i * 2 * a.F + a.F);
-    }
-  }
-  uint32_t wg[8][4], wu[8][4], am = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t d[4] = {d4[i].x, d4[i].y, d4[i].z, d4[i].w}, g[4] = {g4[i].x, g4[i].y, g4[i].z, g4[i].w};
-    const uint32_t u[4] = {u4[i].x, u4[i].y, u4[i].z, u4[i].w};
+    const uint4 g4 = mx_tile_row(buf, i), d4 = mx_tile_row(buf + MX_TILE_BYTES, i), u4 = mx_tile_row(buf + 2 * MX_TILE_BYTES, i);
+    const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       f32x2_t act, grad;
@@ -55,21 +72,33 @@ __global__ void __launch_bounds__(256, 2) gated_grad_kernel(const GatedGradArgs 
       wu[i][j] = f32x2_to_bf16x2(mul2(d2, act));
       wg[i][j] = f32x2_to_bf16x2(mul2(mul2(d2, bf16x2_to_f32x2(u[j])), grad));
     }
-    if (a.dgu != nullptr && f_ok && row + i < a.rows) {
-      *reinterpret_cast<uint4*>(a.dgu + (row + i) * 2 * a.F + f) = make_uint4(wg[i][0], wg[i][1], wg[i][2], wg[i][3]);
-      *reinterpret_cast<uint4*>(a.dgu + (row + i) * 2 * a.F + a.F + f) = make_uint4(wu[i][0], wu[i][1], wu[i][2], wu[i][3]);
+  }
+  __syncwarp();
+  if (lane == 0 && tile + (int)gridDim.x < a.tiles) fetch(tile + gridDim.x);
+  if (a.dgu != nullptr) {
+    const int64_t row = row0 + (lane >> 3) * 8, f = c0 + (lane & 7) * 8;
+    const int nrow = f < a.F ? mx_valid_rows(a.rows, row) : 0;
+    __nv_bfloat16* pg = a.dgu + row * 2 * a.F + f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < nrow) {
+        *reinterpret_cast<uint4*>(pg) = make_uint4(wg[i][0], wg[i][1], wg[i][2], wg[i][3]);
+        *reinterpret_cast<uint4*>(pg + a.F) = make_uint4(wu[i][0], wu[i][1], wu[i][2], wu[i][3]);
+      }
+      pg += 2 * a.F;
     }
   }
   if (a.amax != nullptr) {
+    const bool in = c0 + (lane & 7) * 8 < a.F;   // a tile across the border holds the first columns of u as g
+    uint32_t am = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) am = absmax2(am, absmax2(wu[i][j], wg[i][j]));
-    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, in ? __float_as_uint(absmax2_to_float(am)) : 0u);
     if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
   }
-  const MxTileOut& o = a.out;
-  if (o.q == nullptr) return;
+  if (o.q == nullptr) continue;
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const MxTileScales sc = p ? mx_tile_store(o, wu, row0, a.F + c0, 2 * a.F) : mx_tile_store(o, wg, row0, c0, a.F);
@@ -82,25 +111,30 @@ __global__ void __launch_bounds__(256, 2) gated_grad_kernel(const GatedGradArgs 
     }
   }
   __syncthreads();
-  const int t = tid & 127;
+  const uint32_t t = tid & 127;
+  if (tid < 128) {
+    const uint32_t r = (uint32_t)m0 + t;
+    const int n = (int)min((int64_t)4, (a.F - f0) >> 5);
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    if (tid < 128) {
-      const int64_t b0 = (p ? a.F + f0 : f0) >> 5;
-      const int n = (int)min((int64_t)4, (a.F - f0) >> 5);
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(s_row[p][t]);
-      mx_store_scale_word(word, n, m0 + t < o.rows ? o.s + (m0 + t) * o.s_stride + b0 : nullptr, o.s_swz, m0 + t, b0, o.kc_row);
-    } else if (o.q_t != nullptr && f0 + t < a.F) {
-      const int64_t c = (p ? a.F : 0) + f0 + t, b0 = m0 >> 5;
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(s_col[p][t]);
-      const int n = (int)min((int64_t)4, ((o.rows + 31) >> 5) - b0);
-      mx_store_scale_word(word, n, o.s_t + c * o.s_t_stride + b0, nullptr, c, b0, o.kc_col);
-      mx_store_scale_word(word, 4, nullptr, o.s_t_swz, c, b0, o.kc_col);   // token blocks without a row: zeros
+    for (int p = 0; p < 2; ++p) {
+      const uint32_t b0 = (uint32_t)((p ? a.F + f0 : f0) >> 5);
+      mx_store_scale_word(*reinterpret_cast<const uint32_t*>(s_row[p][t]), n, n == 4 && (b0 & 3) == 0 && row_words,
+                          r < o.rows ? o.s + (uint32_t)(r * (uint32_t)o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
+    }
+  } else if (o.q_t != nullptr && f0 + t < a.F) {
+    const uint32_t b0 = (uint32_t)(m0 >> 5);
+    const int n = (int)min((int64_t)4, ((o.rows + 31) >> 5) - b0);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint32_t c = (uint32_t)((p ? a.F : 0) + f0) + t, word = *reinterpret_cast<const uint32_t*>(s_col[p][t]);
+      mx_store_scale_word(word, n, n == 4 && col_words, o.s_t + (uint32_t)(c * (uint32_t)o.s_t_stride + b0), nullptr, c, b0, 0);
+      // (token blocks without a row: zeros)
+      if (o.s_t_swz != nullptr) *reinterpret_cast<uint32_t*>(o.s_t_swz + mx_swz_offset(c, b0, (uint32_t)o.kc_col)) = word;
     }
   }
   // padding of the GEMM-layout scales: beyond the last feature, and token blocks up to the padded count
   const int64_t mb0 = m0 >> 5, f1 = min(f0 + 128, a.F);
-  const bool last_x = blockIdx.x == gridDim.x - 1, last_y = blockIdx.y == gridDim.y - 1;
+  const bool last_x = tx == a.tiles_x - 1, last_y = tile >= a.tiles - a.tiles_x;
   if (last_x) {
     mx_pad_row_scales(o, m0, 128, tid, 256);
     for (int i = 0; i < 4; ++i) mx_pad_col_features(o, mb0 + i, tid, 256);
@@ -110,6 +144,21 @@ __global__ void __launch_bounds__(256, 2) gated_grad_kernel(const GatedGradArgs 
     mx_pad_col_blocks(o, mb0 + 4, a.F + f0, a.F + f1, tid, 256);
     if (last_x) mx_pad_col_blocks(o, mb0 + 4, 2 * a.F, (2 * a.F + 127) / 128 * 128, tid, 256);
   }
+  __syncthreads();   // the scale bytes have been read
+  }
+}
+
+template <int kAct>
+static int launch_gated_grad(const CUtensorMap& mdh, const CUtensorMap& mgu, const GatedGradArgs& a, cudaStream_t st) {
+  static bool attr_set[MT_MAX_DEVICES] = {};
+  const int slot = current_device_slot();
+  if (!attr_set[slot]) {
+    MT_CUDA(cudaFuncSetAttribute(gated_grad_kernel<kAct>, cudaFuncAttributeMaxDynamicSharedMemorySize, GG_SMEM));
+    attr_set[slot] = true;
+  }
+  const int grid = a.tiles < 2 * mx_sm_count() ? a.tiles : 2 * mx_sm_count();
+  MT_CUDA(launch_pdl(gated_grad_kernel<kAct>, dim3(grid), dim3(256), (size_t)GG_SMEM, st, mdh, mgu, a));
+  return MT_OK;
 }
 
 }  // namespace mt
@@ -120,7 +169,7 @@ extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, const void* 
   using namespace mt;
   const char* name = "mt_gated_backward";
   MT_REQUIRE(rows >= 0 && F >= 0, "%s: negative shape", name);
-  MT_REQUIRE(rows < (int64_t)1 << 23 && F < (int64_t)1 << 30, "%s: shape out of range", name);   // grid.y <= 65535
+  MT_REQUIRE(rows < (int64_t)1 << 30 && F < (int64_t)1 << 29, "%s: shape out of range", name);
   MT_REQUIRE(gated_act_known(activation), "%s: activation %d not supported", name, activation);
   MT_REQUIRE(F % 32 == 0, "%s: F (%lld) must be a multiple of 32", name, (long long)F);
   if (rows == 0 || F == 0) return MT_OK;
@@ -131,14 +180,19 @@ extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, const void* 
   int rc = mx_outputs_ok(name, rows, 2 * F, q, s, s_stride, s_swz, q_t, s_t, s_t_stride, s_t_swz);
   if (rc != MT_OK) return rc;
   GatedGradArgs a{};
-  a.dh = static_cast<const __nv_bfloat16*>(dh); a.gu = static_cast<const __nv_bfloat16*>(gu);
-  a.dh_stride = dh_stride; a.rows = rows; a.F = F;
+  a.rows = rows; a.F = F;
   a.dgu = static_cast<__nv_bfloat16*>(dgu); a.amax = amax;
   a.out = {q, s, s_swz, q_t, s_t, s_t_swz, rows, 2 * F, s_stride, s_t_stride, mx_padded_chunks(2 * F / 32),
            mx_padded_chunks((rows + 31) / 32)};
-  const dim3 grid((unsigned)((F + 127) / 128), (unsigned)((rows + 127) / 128));
+  const int64_t tiles_x = (F + 127) / 128, tiles = tiles_x * ((rows + 127) / 128);
+  MT_REQUIRE(tiles < (int64_t)1 << 30, "%s: shape out of range", name);
+  a.tiles_x = (int)tiles_x; a.tiles = (int)tiles;
+  a.status = device_status_ptr();
+  if (!a.status) return fail(MT_ERR_CUDA, "device status word not reachable");
+  CUtensorMap mdh, mgu;
+  rc = mx_tile_map(&mdh, dh, rows, F, dh_stride);
+  if (rc == MT_OK) rc = mx_tile_map(&mgu, gu, rows, 2 * F, 2 * F);
+  if (rc != MT_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (activation == MT_ACT_SILU) MT_CUDA(launch_pdl(gated_grad_kernel<MT_ACT_SILU>, grid, dim3(256), 0, st, a));
-  else MT_CUDA(launch_pdl(gated_grad_kernel<MT_ACT_GELU>, grid, dim3(256), 0, st, a));
-  return MT_OK;
+  return activation == MT_ACT_SILU ? launch_gated_grad<MT_ACT_SILU>(mdh, mgu, a, st) : launch_gated_grad<MT_ACT_GELU>(mdh, mgu, a, st);
 }

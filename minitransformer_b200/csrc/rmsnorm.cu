@@ -27,32 +27,32 @@ struct RmsNormArgs {
   __nv_bfloat16* y;
   float* amax;
   int cluster;         // CTAs per panel (rmsnorm_panel_kernel)
+  int* status;
   MxTileOut out;
 };
 
 // Order in which both forward kernels add the squares of a row, so that a row's result does not
-// depend on which of them ran: eight columns in turn; the eight such sums of a 64-column segment by a
+// depend on which of them ran: of eight columns the even and the odd ones in turn; the eight such sums of a 64-column segment by a
 // tree over lanes 4, 2, 1 apart; the eight segments of a 512-column group in turn; the groups in turn.
 __device__ __forceinline__ float sum_squares8(const uint4& w) {
-  float s = bf16_lo(w.x) * bf16_lo(w.x);
-  s = fmaf(bf16_hi(w.x), bf16_hi(w.x), s);
-  s = fmaf(bf16_lo(w.y), bf16_lo(w.y), s);
-  s = fmaf(bf16_hi(w.y), bf16_hi(w.y), s);
-  s = fmaf(bf16_lo(w.z), bf16_lo(w.z), s);
-  s = fmaf(bf16_hi(w.z), bf16_hi(w.z), s);
-  s = fmaf(bf16_lo(w.w), bf16_lo(w.w), s);
-  return fmaf(bf16_hi(w.w), bf16_hi(w.w), s);
+  f32x2_t v = bf16x2_to_f32x2(w.x), s = mul2(v, v);
+  v = bf16x2_to_f32x2(w.y); s = fma2(v, v, s);
+  v = bf16x2_to_f32x2(w.z); s = fma2(v, v, s);
+  v = bf16x2_to_f32x2(w.w); s = fma2(v, v, s);
+  float lo, hi;
+  unpack2(s, lo, hi);
+  return lo + hi;
 }
 __device__ __forceinline__ float rstd_of(float sum, int64_t cols, float eps) {
   return __frsqrt_rn(__fdiv_rn(sum, (float)cols) + eps);
 }
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {   // the exact sums, rounded once
+  uint32_t d;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ uint4 add_bf16x8(const uint4& a, const uint4& b) {
-  uint4 o;
-  o.x = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.x), bf16x2_to_f32x2(b.x)));
-  o.y = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.y), bf16x2_to_f32x2(b.y)));
-  o.z = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.z), bf16x2_to_f32x2(b.z)));
-  o.w = f32x2_to_bf16x2(add2(bf16x2_to_f32x2(a.w), bf16x2_to_f32x2(b.w)));
-  return o;
+  return make_uint4(add_bf16x2(a.x, b.x), add_bf16x2(a.y, b.y), add_bf16x2(a.z, b.z), add_bf16x2(a.w, b.w));
 }
 __device__ __forceinline__ void scale_row8(const uint4& w, float rstd, const float (&g)[8], uint32_t (&y)[4]) {
   const f32x2_t r2 = pack2(rstd, rstd);
@@ -93,13 +93,14 @@ __device__ __forceinline__ void load_gamma8(const void* gamma, int is_f32, int64
 // Rows without a transposed copy. One CTA per row, V vectors of 8 columns per thread (vector
 // i * blockDim + thread). The row stays in registers between the sum and the scaling. A 1x32 block is
 // four adjacent lanes. CTAs beyond the last row fill the padding of the GEMM-layout scales with zeros.
-template <int V>
-__global__ void __launch_bounds__(1024) rmsnorm_rows_kernel(const RmsNormArgs a) {
+template <int V, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) rmsnorm_rows_kernel(const RmsNormArgs a) {
   __shared__ float4 seg4[RN_MAX_COLS / 256];   // sums of 64-column segments, a group being two of these
   float* seg = reinterpret_cast<float*>(seg4);
   const MxTileOut& o = a.out;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
+  const bool row_words = mx_word_aligned(o.s, o.s_stride);
   pdl_trigger();
   pdl_wait();
   if (row >= a.rows) {
@@ -156,17 +157,17 @@ __global__ void __launch_bounds__(1024) rmsnorm_rows_kernel(const RmsNormArgs a)
       m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, 2));
       uint32_t f;
-      const uint8_t sb = static_cast<uint8_t>(mx_scale(mx_amax_bits(m), f));
+      uint32_t word = mx_scale(mx_amax_bits(m), f) << (8 * ((tid >> 2) & 3));
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);      // the four blocks of sixteen lanes
       if (on) {
         const float enc = __uint_as_float(f << 16);
         const f32x2_t enc2 = pack2(enc, enc);
         *reinterpret_cast<uint2*>(o.q + row * a.cols + (int64_t)v * 8) =
             make_uint2(e4m3x4_from_words(yw[0], yw[1], enc2), e4m3x4_from_words(yw[2], yw[3], enc2));
-        if ((v & 3) == 0) {
-          const int kb = v >> 2;
-          o.s[row * o.s_stride + kb] = sb;
-          if (o.s_swz != nullptr)
-            o.s_swz[((row >> 7) * o.kc_row + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), kb)] = sb;
+        if ((v & 15) == 0) {
+          const int kb = v >> 2, n = min(4, (nvec >> 2) - kb);
+          mx_store_scale_word(word, n, n == 4 && row_words, o.s + row * o.s_stride + kb, o.s_swz, (uint32_t)row, kb, (uint32_t)o.kc_row);
         }
       }
     }
@@ -180,171 +181,269 @@ __global__ void __launch_bounds__(1024) rmsnorm_rows_kernel(const RmsNormArgs a)
   }
 }
 
-// With a transposed copy. A cluster of C CTAs owns a panel of 32 rows, each CTA 64 columns per warp of
-// it, each warp one 32 x 64 tile in registers (layout of tile_quant.cuh). x is read once: the sums of
-// squares of 512-column groups go to every CTA of the cluster through distributed shared memory,
-// then the tiles are scaled and quantized both ways in place. 32 words of data per thread leave
-// room for 32 warps per SM, enough that some CTAs load while others wait for their cluster or store.
+// With a transposed copy. A cluster of C CTAs owns a panel of 32 rows, each CTA 64 columns per warp of it, each
+// warp one 32 x 64 tile (layout of tile_quant.cuh). x is read once: the sums of squares of 512-column groups go to
+// every CTA of the cluster through distributed shared memory, then the tiles are scaled and quantized both
+// ways in registers. The clusters are persistent: a warp asks for its tiles of the next panel (TMA, one mbarrier
+// per warp) as soon as it holds the present ones, so that they arrive while it waits for its cluster,
+// quantizes and stores. The sums travel by st.async onto an mbarrier of the receiving CTA: a cluster barrier's
+// release would wait for the stores of h, y and the copies as well. Two sets of sums and barriers alternate: a
+// CTA that has received all sums of panel n + 1 knows that everybody has read those of panel n.
 // Panels beyond the last row (up to 128 rows) and the last panel write the scales' padding.
-constexpr int RN_PANEL_MAX_COLS = 16384;
+constexpr int RN_PANEL_MAX_COLS = 8192;
 
-template <int kMaxThreads, int kMinCtas>
-__global__ void __launch_bounds__(kMaxThreads, kMinCtas) rmsnorm_panel_kernel(const RmsNormArgs a) {
-  constexpr int WARPS = kMaxThreads / 32;
-  __shared__ float seg[WARPS][32];                      // this CTA's segments
-  __shared__ float grp[RN_PANEL_MAX_COLS / 512][32];    // the panel's groups
-  __shared__ __align__(16) uint8_t s_row[32][WARPS * 2];
-  const MxTileOut& o = a.out;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  const int cg = lane & 7, rg = lane >> 3;
-  const int rank = (int)cluster_ctarank(), ranks = a.cluster;
-  const int64_t panel = blockIdx.x / ranks, row0 = panel * 32;
-  const int64_t cta_col0 = (int64_t)rank * warps * 64, col0 = cta_col0 + warp * 64;
-  const int64_t r0 = row0 + rg * 8, c = col0 + cg * 8;
-  const bool c_ok = c < a.cols;
-  pdl_trigger();
-  pdl_wait();
-  uint4 w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = make_uint4(0, 0, 0, 0);
-    if (c_ok && r0 + i < a.rows) w[i] = *reinterpret_cast<const uint4*>(a.x + (r0 + i) * a.x_stride + c);
-  }
-  if (a.r != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c_ok && r0 + i < a.rows) {
-        w[i] = add_bf16x8(w[i], *reinterpret_cast<const uint4*>(a.r + (r0 + i) * a.r_stride + c));
-        *reinterpret_cast<uint4*>(a.h + (r0 + i) * a.cols + c) = w[i];
-      }
-  }
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = sum_squares8(w[i]);
-  // eight row sums over eight lanes: every exchange halves the rows a lane still carries
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float send = (cg & 4) ? v[i] : v[i + 4], keep = (cg & 4) ? v[i + 4] : v[i];
-    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float send = (cg & 2) ? v[i] : v[i + 2], keep = (cg & 2) ? v[i + 2] : v[i];
-    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2);
-  }
-  {
-    const float send = (cg & 1) ? v[0] : v[1], keep = (cg & 1) ? v[1] : v[0];
-    v[0] = keep + __shfl_xor_sync(0xffffffffu, send, 1);
-  }
-  seg[warp][lane] = v[0];       // lane l: row l of the panel
-  if (ranks > 1) cluster_arrive();
-  __syncthreads();
-  if (ranks > 1) cluster_wait();   // every CTA of the cluster has started before anything is written into it
-  const int groups = (warps + 7) >> 3;
-  if (warp < groups) {
-    float sum = seg[warp * 8][lane];
-#pragma unroll
-    for (int j = 1; j < 8; ++j)
-      if (warp * 8 + j < warps) sum += seg[warp * 8 + j][lane];
-    const uint32_t mine = smem_u32(&grp[rank * groups + warp][lane]);
-    if (ranks == 1) grp[warp][lane] = sum;
-    else
-      for (int r = 0; r < ranks; ++r)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(mine, (uint32_t)r)), "f"(sum) : "memory");
-  }
-  if (ranks > 1) {
-    cluster_arrive();
-    cluster_wait();
-  } else {
-    __syncthreads();
-  }
-  float total = 0.0f;
-#pragma unroll 4
-  for (int j = 0; j < ranks * groups; ++j) total += grp[j][lane];
-  const float rstd_l = rstd_of(total, a.cols, a.eps);
-  if (rank == 0 && warp == 0 && a.rstd != nullptr && row0 + lane < a.rows) a.rstd[row0 + lane] = rstd_l;
-  if (col0 < a.cols) {          // uniform for the warp
-    float g[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) g[k] = 0.0f;
-    if (c_ok) load_gamma8(a.gamma, a.gamma_f32, c, g);
-    uint32_t yw[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float rs = __shfl_sync(0xffffffffu, rstd_l, rg * 8 + i);
-      if (r0 + i < a.rows) scale_row8(w[i], rs, g, yw[i]);
-      else yw[i][0] = yw[i][1] = yw[i][2] = yw[i][3] = 0;
-      if (a.y != nullptr && c_ok && r0 + i < a.rows)
-        *reinterpret_cast<uint4*>(a.y + (r0 + i) * a.cols + c) = make_uint4(yw[i][0], yw[i][1], yw[i][2], yw[i][3]);
-    }
-    if (a.amax != nullptr) {
-      uint32_t am = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) am = absmax2(am, absmax2(absmax2(yw[i][0], yw[i][1]), absmax2(yw[i][2], yw[i][3])));
-      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
-      if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
-    }
-    const MxTileScales sc = mx_tile_store(o, yw, row0, col0, a.cols);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s_row[rg * 8 + (lane & 3) * 2 + j][warp * 2 + (cg >> 2)] = static_cast<uint8_t>(sc.row[j]);
-      const int64_t f = col0 + cg * 8 + rg * 2 + j;
-      if (f < a.cols) {
-        if (row0 < o.rows) o.s_t[f * o.s_t_stride + panel] = static_cast<uint8_t>(sc.col[j]);
-        if (o.s_t_swz != nullptr)
-          o.s_t_swz[((f >> 7) * o.kc_col + (panel >> 2)) * 512 + sf_chunk_offset((int)(f & 127), (int)(panel & 3))] =
-              static_cast<uint8_t>(sc.col[j]);
+// Bounded wait for data that other CTAs of the cluster send onto a barrier of this one.
+__device__ __forceinline__ void cluster_data_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  const uint64_t t0 = global_timer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return;
+    if ((++spins & 255u) == 0) {
+      if (*abort_flag != 0) return;
+      if (global_timer_ns() - t0 > 2000000000ull) {
+        *abort_flag = 1;
+        atomicOr(status, DS_QUANT_WAIT);
+        return;
       }
     }
-  }
-  __syncthreads();
-  {
-    // row scales: a word (four blocks) per row and pair of warps
-    const int64_t r = row0 + lane, b0 = (cta_col0 >> 5) + warp * 4, nb = a.cols >> 5;
-    if (warp * 2 < warps && b0 < nb) {
-      const int n = (int)min((int64_t)min(4, warps * 2 - warp * 4), nb - b0);
-      uint32_t word = 0;
-      for (int i = 0; i < n; ++i) word |= static_cast<uint32_t>(s_row[lane][warp * 4 + i]) << (8 * i);
-      mx_store_scale_word(word, n, r < o.rows ? o.s + r * o.s_stride + b0 : nullptr, o.s_swz, r, b0, o.kc_row);
-    }
-  }
-  const bool last_rank = rank == ranks - 1;
-  if (last_rank) {
-    mx_pad_row_scales(o, row0, 32, tid, blockDim.x);
-    mx_pad_col_features(o, panel, tid, blockDim.x);
-  }
-  if (panel == gridDim.x / ranks - 1) {
-    const int64_t c0 = min(cta_col0, a.cols), c1 = min(c0 + (int64_t)warps * 64, a.cols);
-    if (c1 > c0) mx_pad_col_blocks(o, panel + 1, c0, c1, tid, blockDim.x);
-    if (last_rank) mx_pad_col_blocks(o, panel + 1, a.cols, (a.cols + 127) / 128 * 128, tid, blockDim.x);
   }
 }
 
-// 512 columns (8 warps) per CTA and up to 8 CTAs per panel; longer rows take 16 or 32 warps per CTA. Groups of 512
-// columns never straddle two CTAs.
-static int launch_rmsnorm_panel(RmsNormArgs& a, cudaStream_t st) {
-  int warps = 8, ranks = (int)((a.cols + 511) / 512);
-  if (a.cols <= 512) warps = (int)((a.cols + 63) / 64);
-  while (ranks > 8) {
-    warps *= 2;
-    ranks = (int)((a.cols + 64 * warps - 1) / (64 * warps));
+template <int kMaxThreads, int kMinCtas>
+__global__ void __launch_bounds__(kMaxThreads, kMinCtas)
+    rmsnorm_panel_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_r, const RmsNormArgs a) {
+  constexpr int WARPS = kMaxThreads / 32;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  __shared__ float seg[WARPS][32];                         // this CTA's segments
+  __shared__ float grp[2][RN_PANEL_MAX_COLS / 512][32];    // the panel's groups; panels alternate
+  __shared__ __align__(16) uint8_t s_row[32][WARPS * 2];
+  __shared__ uint64_t bars[WARPS], xbar[2];
+  __shared__ int abort_flag;
+  const MxTileOut& o = a.out;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int cg = lane & 7, rg = lane >> 3;
+  const int rank = (int)cluster_ctarank(), ranks = a.cluster, groups = (warps + 7) >> 3;
+  const int clusters = gridDim.x / ranks, panels = (int)((a.rows + 127) / 128 * 4);
+  const int64_t cta_col0 = (int64_t)rank * warps * 64, col0 = cta_col0 + warp * 64, c = col0 + cg * 8;
+  const bool w_ok = col0 < a.cols;                         // uniform for the warp
+  uint8_t* buf = smem + warp * 2 * MX_TILE_BYTES;
+  const bool row_words = mx_word_aligned(o.s, o.s_stride);
+  const bool pad_cols = rank == ranks - 1 && (a.cols & 511) != 0;   // GEMM-layout scales go beyond the last column
+  if (tid == 0) {
+    abort_flag = 0;
+    mbar_init(&xbar[0], 1);
+    mbar_init(&xbar[1], 1);
   }
-  a.cluster = ranks;
+  if (lane == 0) mbar_init(&bars[warp], 1);
+  mbar_fence_init();
+  __syncthreads();
+  if (ranks > 1) {   // every CTA's barriers exist before anything is sent to it
+    cluster_arrive();
+    cluster_wait();
+  }
+  pdl_wait();
+  float g[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) g[k] = 0.0f;
+  if (c < a.cols) load_gamma8(a.gamma, a.gamma_f32, c, g);
+  auto fetch = [&](int panel) {
+    mbar_expect_tx(&bars[warp], (a.r != nullptr ? 2 : 1) * MX_TILE_BYTES);
+    tma_load_2d(buf, &map_x, &bars[warp], (int32_t)col0, panel * 32);
+    if (a.r != nullptr) tma_load_2d(buf + MX_TILE_BYTES, &map_r, &bars[warp], (int32_t)col0, panel * 32);
+  };
+  if (lane == 0 && w_ok && (int)blockIdx.x / ranks < panels) fetch(blockIdx.x / ranks);
+  uint32_t turn = 0;
+  for (int panel = blockIdx.x / ranks; panel < panels; panel += clusters, ++turn) {
+    const int64_t row0 = (int64_t)panel * 32, r0 = row0 + rg * 8;
+    const int nrow = c < a.cols ? mx_valid_rows(a.rows, r0) : 0;
+    uint4 w[8];
+    if (w_ok) {
+      // on expiry the status word tells; the warp goes on with what is there, so that nobody waits for it
+      mbar_wait_bounded(&bars[warp], turn & 1, &abort_flag, a.status, DS_QUANT_WAIT);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = mx_tile_row(buf, i);
+      if (a.r != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = add_bf16x8(w[i], mx_tile_row(buf + MX_TILE_BYTES, i));
+      }
+      __syncwarp();
+      if (lane == 0 && panel + clusters < panels) fetch(panel + clusters);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = sum_squares8(w[i]);
+    // eight row sums over eight lanes: every exchange halves the rows a lane still carries
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float send = (cg & 4) ? v[i] : v[i + 4], keep = (cg & 4) ? v[i + 4] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float send = (cg & 2) ? v[i] : v[i + 2], keep = (cg & 2) ? v[i + 2] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2);
+    }
+    {
+      const float send = (cg & 1) ? v[0] : v[1], keep = (cg & 1) ? v[1] : v[0];
+      v[0] = keep + __shfl_xor_sync(0xffffffffu, send, 1);
+    }
+    seg[warp][lane] = v[0];       // lane l: row l of the panel
+    __syncthreads();
+    if (warp < groups) {
+      float sum = seg[warp * 8][lane];
+#pragma unroll
+      for (int j = 1; j < 8; ++j)
+        if (warp * 8 + j < warps) sum += seg[warp * 8 + j][lane];
+      float* mine = &grp[turn & 1][rank * groups + warp][lane];
+      if (ranks == 1) *mine = sum;
+      else {
+        if (tid == 0) mbar_expect_tx(&xbar[turn & 1], (uint32_t)(ranks * groups) * 128);
+        for (int r = 0; r < ranks; ++r)
+          asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                       ::"r"(map_to_cta(smem_u32(mine), (uint32_t)r)), "r"(__float_as_uint(sum)),
+                         "r"(map_to_cta(smem_u32(&xbar[turn & 1]), (uint32_t)r)) : "memory");
+      }
+    }
+    if (ranks > 1) cluster_data_wait(&xbar[turn & 1], (turn >> 1) & 1, &abort_flag, a.status);
+    else __syncthreads();
+    float total = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < ranks * groups; ++j) total += grp[turn & 1][j][lane];
+    const bool live = row0 + lane < a.rows;
+    const float rstd_l = live ? rstd_of(total, a.cols, a.eps) : 0.0f;
+    if (rank == 0 && warp == 0 && a.rstd != nullptr && live) a.rstd[row0 + lane] = rstd_l;
+    if (w_ok) {
+      if (a.h != nullptr) {
+        __nv_bfloat16* p = a.h + r0 * a.cols + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i < nrow) *reinterpret_cast<uint4*>(p) = w[i];
+          p += a.cols;
+        }
+      }
+      uint32_t yw[8][4];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)    // (rows beyond the last are zeros)
+        scale_row8(w[i], __shfl_sync(0xffffffffu, rstd_l, rg * 8 + i), g, yw[i]);
+      if (a.y != nullptr) {
+        __nv_bfloat16* p = a.y + r0 * a.cols + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i < nrow) *reinterpret_cast<uint4*>(p) = make_uint4(yw[i][0], yw[i][1], yw[i][2], yw[i][3]);
+          p += a.cols;
+        }
+      }
+      if (a.amax != nullptr) {
+        uint32_t am = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) am = absmax2(am, absmax2(absmax2(yw[i][0], yw[i][1]), absmax2(yw[i][2], yw[i][3])));
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
+        if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
+      }
+      const MxTileScales sc = mx_tile_store(o, yw, row0, col0, a.cols);
+      const uint32_t f0 = (uint32_t)col0 + cg * 8 + rg * 2;    // two adjacent features: both inside or both outside
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        s_row[rg * 8 + (lane & 3) * 2 + j][warp * 2 + (cg >> 2)] = static_cast<uint8_t>(sc.row[j]);
+      if (f0 < a.cols) {
+        const uint32_t stride = (uint32_t)o.s_t_stride;
+        if (row0 < o.rows) {
+          uint8_t* lin = o.s_t + (f0 * stride + panel);
+          lin[0] = static_cast<uint8_t>(sc.col[0]);
+          lin[stride] = static_cast<uint8_t>(sc.col[1]);
+        }
+        if (o.s_t_swz != nullptr) {
+          uint8_t* swz = o.s_t_swz + mx_swz_offset(f0, panel, (uint32_t)o.kc_col);
+          swz[0] = static_cast<uint8_t>(sc.col[0]);
+          swz[16] = static_cast<uint8_t>(sc.col[1]);
+        }
+      }
+    }
+    __syncthreads();
+    if (warp * 2 < warps) {
+      // row scales: a word (four blocks) per row and pair of warps
+      const uint32_t r = (uint32_t)row0 + lane, b0 = (uint32_t)(cta_col0 >> 5) + warp * 4;
+      const int n = min(min(4, warps * 2 - warp * 4), (int)(a.cols >> 5) - (int)b0);
+      if (n > 0)
+        mx_store_scale_word(*reinterpret_cast<const uint32_t*>(&s_row[lane][warp * 4]), n, n == 4 && row_words,
+                            live ? o.s + (uint32_t)(r * (uint32_t)o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
+    }
+    if (pad_cols) {
+      mx_pad_row_scales(o, row0, 32, tid, blockDim.x);
+      mx_pad_col_features(o, panel, tid, blockDim.x);
+    }
+    if (panel == panels - 1) {
+      const int64_t c0 = min(cta_col0, a.cols), c1 = min(c0 + (int64_t)warps * 64, a.cols);
+      if (c1 > c0) mx_pad_col_blocks(o, panel + 1, c0, c1, tid, blockDim.x);
+      if (pad_cols) mx_pad_col_blocks(o, panel + 1, a.cols, (a.cols + 127) / 128 * 128, tid, blockDim.x);
+    }
+  }
+  if (ranks > 1) {   // nobody leaves while something may still be on its way to it
+    cluster_arrive();
+    cluster_wait();
+  }
+  // only now: with clusters of the next kernel taking their places earlier, calls in a row took 104 us instead of 81
+  pdl_trigger();
+}
+
+// 512 columns (8 warps) per CTA and up to 8 CTAs per panel; longer rows take 16 warps per CTA. Groups of 512 columns
+// never straddle two CTAs.
+template <int kMaxThreads, int kMinCtas>
+static int launch_rmsnorm_panel(RmsNormArgs& a, int warps, int ranks, cudaStream_t st) {
+  CUtensorMap mx, mr;
+  int rc = mx_tile_map(&mx, a.x, a.rows, a.cols, a.x_stride);
+  if (rc == MT_OK) rc = a.r ? mx_tile_map(&mr, a.r, a.rows, a.cols, a.r_stride) : (mr = mx, MT_OK);
+  if (rc != MT_OK) return rc;
+  auto kern = rmsnorm_panel_kernel<kMaxThreads, kMinCtas>;
+  const size_t smem = (size_t)warps * 2 * MX_TILE_BYTES + 128;
+  static int max_clusters_dev[MT_MAX_DEVICES][9] = {};   // by cluster size, for the full number of warps
+  int& max_clusters = max_clusters_dev[current_device_slot()][ranks];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.rows + 127) / 128 * 4 * ranks));
-  cfg.blockDim = dim3(32 * warps);
-  cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  if (max_clusters <= 0) {
+    const size_t most = (size_t)(kMaxThreads / 32) * 2 * MX_TILE_BYTES + 128;
+    MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    cfg.gridDim = dim3(ranks * 1024);
+    cfg.blockDim = dim3(kMaxThreads);
+    cfg.dynamicSmemBytes = most;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) { cudaGetLastError(); n = mx_sm_count() / ranks; }
+    max_clusters = n > 0 ? n : 1;
+  }
+  const int64_t panels = (a.rows + 127) / 128 * 4;
+  a.cluster = ranks;
+  cfg.gridDim = dim3((unsigned)((panels < max_clusters ? panels : max_clusters) * ranks));
+  cfg.blockDim = dim3(32 * warps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   const RmsNormArgs& ca = a;
-  if (warps <= 8) MT_CUDA(cudaLaunchKernelEx(&cfg, rmsnorm_panel_kernel<256, 4>, ca));
-  else MT_CUDA(cudaLaunchKernelEx(&cfg, rmsnorm_panel_kernel<1024, 1>, ca));
+  MT_CUDA(cudaLaunchKernelEx(&cfg, kern, mx, mr, ca));
   return MT_OK;
+}
+
+static int rmsnorm_panel(RmsNormArgs& a, cudaStream_t st) {
+  a.status = device_status_ptr();
+  if (!a.status) return fail(MT_ERR_CUDA, "device status word not reachable");
+  if (a.cols <= 512) return launch_rmsnorm_panel<256, 2>(a, (int)((a.cols + 63) / 64), 1, st);
+  if (a.cols <= 4096) return launch_rmsnorm_panel<256, 2>(a, 8, (int)((a.cols + 511) / 512), st);
+  return launch_rmsnorm_panel<512, 1>(a, 16, (int)((a.cols + 1023) / 1024), st);
 }
 
 // ---- gradient ----
@@ -457,23 +556,11 @@ __global__ void __launch_bounds__(256) rmsnorm_dgamma_kernel(const float* partia
   }
 }
 
-static int rn_sm_count() {
-  static int n[MT_MAX_DEVICES] = {};
-  const int slot = current_device_slot();
-  if (n[slot] == 0) {
-    int dev = 0, c = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
-    n[slot] = c > 0 ? c : 148;
-  }
-  return n[slot];
-}
-
 // Threads per row for V vectors per thread (a multiple of 64: whole groups of four segments).
 static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / V + 63) / 64 * 64); }
 
 static int rn_grad_ctas(int64_t rows) {
-  const int64_t most = 2 * (int64_t)rn_sm_count();
+  const int64_t most = 2 * (int64_t)mx_sm_count();
   return (int)(rows < most ? rows : most);
 }
 
@@ -513,11 +600,14 @@ extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* r
            mx_padded_chunks((rows + 31) / 32)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t padded = (rows + 127) / 128 * 128;
-  if (q_t) return launch_rmsnorm_panel(a, st);
+  if (q_t) return rmsnorm_panel(a, st);
   const dim3 grid((unsigned)(s_swz ? padded : rows));
-  if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<1>, grid, dim3(rn_threads(cols, 1)), 0, st, a));
-  else if (cols <= 16384) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<2>, grid, dim3(rn_threads(cols, 2)), 0, st, a));
-  else MT_CUDA(launch_pdl(rmsnorm_rows_kernel<4>, grid, dim3(rn_threads(cols, 4)), 0, st, a));
+  // Few rows: one vector per thread, the shortest way through a row. Many rows: four vectors per thread, so that more
+  // rows (and bytes) are in flight per SM: 8192 x 4096 with a residual takes 54 us with one vector, XX with four.
+  const bool many = rows >= 4 * mx_sm_count();
+  if (cols <= 8192 && !many) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<1, 1024>, grid, dim3(rn_threads(cols, 1)), 0, st, a));
+  else if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<4, 256>, grid, dim3(rn_threads(cols, 4)), 0, st, a));
+  else MT_CUDA(launch_pdl(rmsnorm_rows_kernel<4, 1024>, grid, dim3(rn_threads(cols, 4)), 0, st, a));
   return MT_OK;
 }
 

@@ -37,6 +37,25 @@ static inline int mx_outputs_ok(const char* name, int64_t rows, int64_t cols, co
   return MT_OK;
 }
 
+constexpr int MX_TILE_BYTES = 32 * 128;
+// Tensor map of a bf16 matrix read in 32 x 64 tiles (zeros beyond its bounds).
+static inline int mx_tile_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t stride) {
+  return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, (uint64_t)cols, (uint64_t)rows, (uint64_t)stride * 2, 64,
+                            32, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+// Streaming multiprocessors of the current device.
+static inline int mx_sm_count() {
+  static int n[MT_MAX_DEVICES] = {};
+  const int slot = current_device_slot();
+  if (n[slot] == 0) {
+    int dev = 0, c = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
+    n[slot] = c > 0 ? c : 148;
+  }
+  return n[slot];
+}
+
 #if defined(__CUDACC__)
 
 // Scale of a block from the bits of its abs-max as bf16 (sign cleared): E8M0 byte and the factor 2^-e that the
@@ -74,6 +93,26 @@ struct MxTileScales {
   uint32_t row[2], col[2];
 };
 
+// A warp's 32 x 64 bf16 tile as TMA leaves it (rows of 128 bytes): this lane's 16 bytes of row i.
+__device__ __forceinline__ uint4 mx_tile_row(const uint8_t* tile, int i) {
+  const int lane = threadIdx.x & 31;
+  return *reinterpret_cast<const uint4*>(tile + ((lane >> 3) * 8 + i) * 128 + (lane & 7) * 16);
+}
+
+// Rows of [row, row + 8) below `rows`.
+__device__ __forceinline__ int mx_valid_rows(int64_t rows, int64_t row) {
+  return (int)max((int64_t)0, min((int64_t)8, rows - row));
+}
+// The first n of eight bytes, anywhere.
+__device__ __forceinline__ void mx_store_bytes(uint8_t* dst, uint2 v, int n) {
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    dst[i] = static_cast<uint8_t>(v.x);
+    v.x = __funnelshift_r(v.x, v.y, 8);
+    v.y >>= 8;
+  }
+}
+
 // Codes of the tile -> global memory. row0 / col0: its first row and column (multiples of 32). Columns from
 // `limit` on are not stored; rows beyond o.rows hold zeros. A column block is whole or absent (limit % 32 == 0).
 // The abs-max of a block is reduced over its four lanes so that every exchange halves the number of rows (or
@@ -84,6 +123,7 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
   const int lane = threadIdx.x & 31, cg = lane & 7, rg = lane >> 3;
   const int64_t row = row0 + rg * 8, col = col0 + cg * 8;
   const bool col_ok = col < limit;
+  const int nrow = col_ok ? mx_valid_rows(o.rows, row) : 0;   // rows of this lane that are stored
   MxTileScales sc;
   // ---- rows ----
   {
@@ -115,9 +155,10 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
         uint32_t v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = mul_bf16x2(w[i][k], f);
-        if (col_ok && row + i < o.rows)
-          *reinterpret_cast<uint2*>(dst + i * o.cols) = make_uint2(e4m3x4_rn(bf16_lo(v[0]), bf16_hi(v[0]), bf16_lo(v[1]), bf16_hi(v[1])),
-                                                                   e4m3x4_rn(bf16_lo(v[2]), bf16_hi(v[2]), bf16_lo(v[3]), bf16_hi(v[3])));
+        if (i < nrow)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(e4m3x4_rn(bf16_lo(v[0]), bf16_hi(v[0]), bf16_lo(v[1]), bf16_hi(v[1])),
+                                                      e4m3x4_rn(bf16_lo(v[2]), bf16_hi(v[2]), bf16_lo(v[3]), bf16_hi(v[3])));
+        dst += o.cols;
       }
     }
   }
@@ -144,6 +185,7 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
   sc.col[1] = mx_scale((m[0] >> 16) & 0x7FFFu, e1);
   const uint32_t pair = e0 | (e1 << 16);
   const bool vec = (o.rows & 7) == 0;
+  uint8_t* dst = o.q_t + col * o.rows + row;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t f = __shfl_sync(0xffffffffu, pair, j * 8 + cg);
@@ -154,46 +196,41 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
                                 e4m3x4_rn(bf16_lo(v[4]), bf16_lo(v[5]), bf16_lo(v[6]), bf16_lo(v[7])));
     const uint2 hi = make_uint2(e4m3x4_rn(bf16_hi(v[0]), bf16_hi(v[1]), bf16_hi(v[2]), bf16_hi(v[3])),
                                 e4m3x4_rn(bf16_hi(v[4]), bf16_hi(v[5]), bf16_hi(v[6]), bf16_hi(v[7])));
-    if (col_ok) {
-      uint8_t* dst = o.q_t + (col + 2 * j) * o.rows + row;
-      if (vec) {
-        if (row < o.rows) {
-          *reinterpret_cast<uint2*>(dst) = lo;
-          *reinterpret_cast<uint2*>(dst + o.rows) = hi;
-        }
-      } else {
-        const int n = (int)min((int64_t)8, o.rows - row);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i < n) {
-            dst[i] = static_cast<uint8_t>((i < 4 ? lo.x : lo.y) >> (8 * (i & 3)));
-            dst[o.rows + i] = static_cast<uint8_t>((i < 4 ? hi.x : hi.y) >> (8 * (i & 3)));
-          }
-        }
-      }
+    if (vec) {                       // then a lane has all of its rows or none
+      if (nrow > 0) *reinterpret_cast<uint2*>(dst) = lo;
+      dst += o.rows;
+      if (nrow > 0) *reinterpret_cast<uint2*>(dst) = hi;
+    } else {
+      mx_store_bytes(dst, lo, nrow);
+      dst += o.rows;
+      mx_store_bytes(dst, hi, nrow);
     }
+    dst += o.rows;
   }
   return sc;
 }
 
-// The bytes of a scale word (blocks b0 .. b0 + 3 of one row, b0 % 4 == 0 unless n < 4): the first n of them to the
-// row-major scales (`lin`, at block b0) and the GEMM layout (`swz`, nb chunks per 128 rows).
-__device__ __forceinline__ void mx_store_scale_word(uint32_t word, int n, uint8_t* lin, uint8_t* swz, int64_t row, int64_t b0,
-                                                    int64_t kc) {
-  if (lin != nullptr) {
-    if (n == 4 && (reinterpret_cast<uintptr_t>(lin) & 3) == 0) *reinterpret_cast<uint32_t*>(lin) = word;
-    else
-      for (int i = 0; i < n; ++i) lin[i] = static_cast<uint8_t>(word >> (8 * i));
+// Byte offset of the scale of (row, block) in a GEMM layout of kc chunks per 128 rows. 32 bits reach 128 G elements.
+__device__ __forceinline__ uint32_t mx_swz_offset(uint32_t row, uint32_t block, uint32_t kc) {
+  return ((row >> 7) * kc + (block >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)(block & 3));
+}
+// The first n scale bytes of `word` (blocks b0 .. of one row) to their places in a row-major row (lin, null: none)
+// and in the GEMM layout (swz, null: none); `whole`: n == 4, b0 % 4 == 0 and lin 4-byte aligned (uniform).
+__device__ __forceinline__ void mx_store_scale_word(uint32_t word, int n, bool whole, uint8_t* lin, uint8_t* swz, uint32_t row,
+                                                    uint32_t b0, uint32_t kc) {
+  if (whole) {
+    if (lin != nullptr) *reinterpret_cast<uint32_t*>(lin) = word;
+    if (swz != nullptr) *reinterpret_cast<uint32_t*>(swz + mx_swz_offset(row, b0, kc)) = word;
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i, word >>= 8) {
+      if (lin != nullptr) lin[i] = static_cast<uint8_t>(word);
+      if (swz != nullptr) swz[mx_swz_offset(row, b0 + i, kc)] = static_cast<uint8_t>(word);
+    }
   }
-  if (swz != nullptr) {
-    if (n == 4 && (b0 & 3) == 0)
-      *reinterpret_cast<uint32_t*>(swz + ((row >> 7) * kc + (b0 >> 2)) * 512 + sf_chunk_offset((int)(row & 127), 0)) = word;
-    else
-      for (int i = 0; i < n; ++i) {
-        const int64_t b = b0 + i;
-        swz[((row >> 7) * kc + (b >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)(b & 3))] = static_cast<uint8_t>(word >> (8 * i));
-      }
-  }
+}
+__device__ __forceinline__ bool mx_word_aligned(const void* p, int64_t stride) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride) & 3) == 0;
 }
 
 // Zeros of the GEMM-layout scales that no tile covers: blocks beyond the last column (for `nrows` rows from

@@ -576,7 +576,7 @@ def _mxfp8_outputs(rows: int, cols: int, transpose: bool, device) -> Quantized:
 
 
 _NO_COPIES = Quantized(None, None, None)
-_NORM_PANEL_COLS = 16384     # columns up to which mt_rmsnorm_forward makes a transposed copy
+_NORM_PANEL_COLS = 8192     # columns up to which mt_rmsnorm_forward makes a transposed copy
 
 
 @dataclass

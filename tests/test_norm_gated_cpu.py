@@ -52,7 +52,7 @@ def test_norm_entry_points_refuse(p):
     _refused(fwd(q=p, s=p, qt=p, st=p, sts=0), "need s_t")
     _refused(fwd(q=p, s=p, st=p), "without transposed codes")
     _refused(fwd(qt=p, st=p), "without codes")
-    assert fwd(cols=16416, xs=16416, q=p, s=p, ss=513, qt=p, st=p) == -2
+    assert fwd(cols=8224, xs=8224, q=p, s=p, ss=257, qt=p, st=p) == -2
     _refused(fwd(q=p + 8, s=p), "16-byte")
     _refused(fwd(s=p), "without codes")
     assert fwd(rows=0, x=None) == 0                 # nothing to do
@@ -115,7 +115,7 @@ def test_gated_entry_points_refuse(p):
     _refused(gb(q=p, s=p, st=p), "without transposed codes")
     _refused(gb(qt=p, st=p), "without codes")
     _refused(gb(q=p + 8, s=p), "16-byte")
-    _refused(gb(rows=1 << 23), "out of range")
+    _refused(gb(rows=1 << 40), "out of range")
 
     _refused(gb(F=40), "multiple of 32")
     _refused(gb(act=5), "activation")
