@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256, 2)
     gated_grad_kernel(const __grid_constant__ CUtensorMap map_dh, const __grid_constant__ CUtensorMap map_gu, const GatedGradArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
-  __shared__ __align__(16) uint8_t s_row[2][128][4], s_col[2][128][4];   // [dg, du][row / feature][block]
+  __shared__ __align__(16) uint8_t s_rows[2][2][128][4], s_cols[2][2][128][4];   // [turn][dg, du][row / feature][block]
   __shared__ uint64_t bars[8];
   __shared__ int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -40,7 +40,6 @@ __global__ void __launch_bounds__(256, 2)
   if (lane == 0) mbar_init(&bars[warp], 1);
   mbar_fence_init();
   __syncthreads();
-  pdl_trigger();
   pdl_wait();
 
   auto fetch = [&](int tile) {
@@ -57,6 +56,7 @@ __global__ void __launch_bounds__(256, 2)
   const int ty = tile / a.tiles_x, tx = tile - ty * a.tiles_x;
   const int64_t m0 = (int64_t)ty * 128, f0 = (int64_t)tx * 128;
   const int64_t row0 = m0 + wr * 32, c0 = f0 + wc * 64;
+  uint8_t (&s_row)[2][128][4] = s_rows[ph], (&s_col)[2][128][4] = s_cols[ph];   // turns alternate: one barrier each
   // on expiry the status word tells; the warp goes on with what is there, so that nobody waits for it
   mbar_wait_bounded(&bars[warp], ph, &abort_flag, a.status, DS_QUANT_WAIT);
   uint32_t wg[8][4], wu[8][4];
@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(256, 2)
     mx_pad_col_blocks(o, mb0 + 4, a.F + f0, a.F + f1, tid, 256);
     if (last_x) mx_pad_col_blocks(o, mb0 + 4, 2 * a.F, (2 * a.F + 127) / 128 * 128, tid, 256);
   }
-  __syncthreads();   // the scale bytes have been read
   }
+  pdl_trigger();
 }
 
 template <int kAct>
