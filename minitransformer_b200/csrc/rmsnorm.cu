@@ -90,42 +90,17 @@ __device__ __forceinline__ void load_gamma8(const void* gamma, int is_f32, int64
   }
 }
 
-// Rows without a transposed copy. One CTA per row, V vectors of 8 columns per thread (vector
-// i * blockDim + thread). The row stays in registers between the sum and the scaling. A 1x32 block is
-// four adjacent lanes. CTAs beyond the last row fill the padding of the GEMM-layout scales with zeros.
-template <int V, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) rmsnorm_rows_kernel(const RmsNormArgs a) {
-  __shared__ float4 seg4[RN_MAX_COLS / 256];   // sums of 64-column segments, a group being two of these
+// Sum of squares of the row that the CTA holds, the same in every thread; one barrier. `seg4` belongs to this row until
+// the barrier of the next one.
+template <int V>
+__device__ __forceinline__ float rmsnorm_row_sum(const uint4 (&w)[V], float4* seg4) {
   float* seg = reinterpret_cast<float*>(seg4);
-  const MxTileOut& o = a.out;
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
-  const bool row_words = mx_word_aligned(o.s, o.s_stride);
-  pdl_trigger();
-  pdl_wait();
-  if (row >= a.rows) {
-    uint8_t* cell = o.s_swz + (row >> 7) * o.kc_row * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
-    for (int64_t c = tid; c < o.kc_row; c += blockDim.x) *reinterpret_cast<uint32_t*>(cell + c * 512) = 0u;
-    return;
-  }
-  uint4 w[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int v = i * blockDim.x + tid;
-    w[i] = make_uint4(0, 0, 0, 0);
-    if (v < nvec) {
-      w[i] = *reinterpret_cast<const uint4*>(a.x + row * a.x_stride + (int64_t)v * 8);
-      if (a.r != nullptr) w[i] = add_bf16x8(w[i], *reinterpret_cast<const uint4*>(a.r + row * a.r_stride + (int64_t)v * 8));
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int v = i * blockDim.x + tid;
-    if (a.h != nullptr && v < nvec) *reinterpret_cast<uint4*>(a.h + row * a.cols + (int64_t)v * 8) = w[i];
     float ss = sum_squares8(w[i]);
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    if ((tid & 7) == 0) seg[v >> 3] = ss;      // (V * blockDim) / 8 segments, zeros beyond the row
+    if ((threadIdx.x & 7) == 0) seg[(i * blockDim.x + threadIdx.x) >> 3] = ss;   // zeros beyond the row
   }
   __syncthreads();
   const int groups = (int)(V * blockDim.x) >> 6;   // blockDim is a multiple of 64
@@ -135,10 +110,20 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_rows_kernel(const RmsNorm
     const float4 p = seg4[2 * j], u = seg4[2 * j + 1];
     total += ((((((p.x + p.y) + p.z) + p.w) + u.x) + u.y) + u.z) + u.w;
   }
-  const float rstd = rstd_of(total, a.cols, a.eps);
-  if (tid == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
+  return total;
+}
+// Scales of rows that the GEMM layout pads to 128.
+__device__ __forceinline__ void rmsnorm_pad_row(const MxTileOut& o, int64_t row) {
+  uint8_t* cell = o.s_swz + (row >> 7) * o.kc_row * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+  for (int64_t c = threadIdx.x; c < o.kc_row; c += blockDim.x) *reinterpret_cast<uint32_t*>(cell + c * 512) = 0u;
+}
 
-  uint32_t am = 0;
+// A row in registers, its rstd known: y, codes, scales, and the row's abs-max into am.
+template <int V>
+__device__ __forceinline__ void rmsnorm_finish_row(const RmsNormArgs& a, const uint4 (&w)[V], int64_t row, float rstd, bool row_words,
+                                                   uint32_t& am) {
+  const MxTileOut& o = a.out;
+  const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = i * blockDim.x + tid;
@@ -175,10 +160,49 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_rows_kernel(const RmsNorm
   if (o.s_swz != nullptr)   // blocks beyond the row, up to the padded chunk count
     for (int64_t kb = (a.cols >> 5) + tid; kb < o.kc_row * 4; kb += blockDim.x)
       o.s_swz[((row >> 7) * o.kc_row + (kb >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)kb)] = 0;
+}
+__device__ __forceinline__ void rmsnorm_publish_amax(const RmsNormArgs& a, uint32_t am) {
   if (a.amax != nullptr) {
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
-    if ((tid & 31) == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
+    if ((threadIdx.x & 31) == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
   }
+}
+
+// Rows without a transposed copy. One CTA per row, V vectors of 8 columns per thread (vector
+// i * blockDim + thread). The row stays in registers between the sum and the scaling. A 1x32 block is
+// four adjacent lanes. CTAs beyond the last row fill the padding of the GEMM-layout scales with zeros.
+template <int V, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) rmsnorm_rows_kernel(const RmsNormArgs a) {
+  __shared__ float4 seg4[RN_MAX_COLS / 256];   // sums of 64-column segments, a group being two of these
+  const MxTileOut& o = a.out;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, nvec = (int)(a.cols >> 3);
+  pdl_trigger();
+  pdl_wait();
+  if (row >= a.rows) {
+    rmsnorm_pad_row(o, row);
+    return;
+  }
+  uint4 w[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (v < nvec) {
+      w[i] = *reinterpret_cast<const uint4*>(a.x + row * a.x_stride + (int64_t)v * 8);
+      if (a.r != nullptr) w[i] = add_bf16x8(w[i], *reinterpret_cast<const uint4*>(a.r + row * a.r_stride + (int64_t)v * 8));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    if (a.h != nullptr && v < nvec) *reinterpret_cast<uint4*>(a.h + row * a.cols + (int64_t)v * 8) = w[i];
+  }
+  const float rstd = rstd_of(rmsnorm_row_sum<V>(w, seg4), a.cols, a.eps);
+  if (tid == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
+  uint32_t am = 0;
+  rmsnorm_finish_row<V>(a, w, row, rstd, mx_word_aligned(o.s, o.s_stride), am);
+  rmsnorm_publish_amax(a, am);
 }
 
 // With a transposed copy. A cluster of C CTAs owns a panel of 32 rows, each CTA 64 columns per warp of it, each
@@ -449,6 +473,10 @@ static int rmsnorm_panel(RmsNormArgs& a, cudaStream_t st) {
 // ---- gradient ----
 //   a = dy * gamma, xhat = h * rstd
 //   dx = rstd * (a - xhat * mean_k(a * xhat)) (+ dres),   dgamma = sum_rows dy * xhat
+constexpr int RN_RING_STAGES = 8;
+constexpr int RN_RING_MAX_COLS = 16384;
+constexpr int RN_RING_BYTES = 200 * 1024;   // shared memory per SM that the rings share
+
 struct RmsNormGradArgs {
   const __nv_bfloat16 *dy, *h, *dres;
   int64_t dy_stride, h_stride, dres_stride;
@@ -458,6 +486,8 @@ struct RmsNormGradArgs {
   int64_t rows, cols;
   __nv_bfloat16* dx;
   float* partial;   // [gridDim.x, cols]
+  int stages;       // of the ring
+  int* status;
 };
 
 // Persistent CTAs over rows; a thread keeps the same columns for every row, so the column sums
@@ -537,21 +567,126 @@ __global__ void __launch_bounds__(1024) rmsnorm_grad_kernel(const RmsNormGradArg
   }
 }
 
-// dgamma[k] = sum of `parts` partial rows, in order. 32 columns per CTA, 8 row groups.
-__global__ void __launch_bounds__(256) rmsnorm_dgamma_kernel(const float* partial, int parts, int64_t cols, float* dgamma) {
-  __shared__ float sum[8][32];
+// The same with the rows on their way ahead of time: a ring of shared-memory stages, each one row of dy, h and dres
+// fetched by bulk copies (one mbarrier per stage). A row needs one barrier (inside the sum); once a thread
+// has passed the one of row n + 1, everybody is done with row n, and its stage is filled again.
+template <int V, int kMaxThreads, int kMinCtas>
+__global__ void __launch_bounds__(kMaxThreads, kMinCtas) rmsnorm_grad_ring_kernel(const RmsNormGradArgs a) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float slot[2][32];
+  __shared__ uint64_t full[RN_RING_STAGES];
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, nvec = (int)(a.cols >> 3), stages = a.stages;
+  const uint32_t row_bytes = (uint32_t)a.cols * 2, stage_bytes = row_bytes * (a.dres != nullptr ? 3 : 2);
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  auto fetch = [&](int64_t row, int s) {
+    uint8_t* p = ring + s * stage_bytes;
+    mbar_expect_tx(&full[s], stage_bytes);
+    bulk_load_1d(p, a.dy + row * a.dy_stride, row_bytes, &full[s]);
+    bulk_load_1d(p + row_bytes, a.h + row * a.h_stride, row_bytes, &full[s]);
+    if (a.dres != nullptr) bulk_load_1d(p + 2 * row_bytes, a.dres + row * a.dres_stride, row_bytes, &full[s]);
+  };
+  if (tid == 0)
+    for (int i = 0; i < stages; ++i) {
+      const int64_t row = blockIdx.x + (int64_t)i * gridDim.x;
+      if (row < a.rows) fetch(row, i);
+    }
+  float g[V][8], acc[V][8];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[i][j] = acc[i][j] = 0.0f;
+    if (i * (int)blockDim.x + tid < nvec) load_gamma8(a.gamma, a.gamma_f32, (int64_t)(i * blockDim.x + tid) * 8, g[i]);
+  }
+  const float inv = __fdiv_rn(1.0f, (float)a.cols);
+  int s = 0, turn = 0, last = 0;
+  uint32_t ph = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const uint8_t* p = ring + s * stage_bytes;
+    const float rstd = a.rstd[row];
+    // on expiry the status word tells; the CTA goes on with what is there
+    mbar_wait_bounded(&full[s], ph, &abort_flag, a.status, DS_QUANT_WAIT);
+    f32x2_t dot2 = pack2(0.0f, 0.0f);
+    uint4 dy[V], h[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = i * blockDim.x + tid;
+      dy[i] = h[i] = make_uint4(0, 0, 0, 0);
+      if (v < nvec) {
+        dy[i] = *reinterpret_cast<const uint4*>(p + v * 16);
+        h[i] = *reinterpret_cast<const uint4*>(p + row_bytes + v * 16);
+      }
+      const uint32_t d[4] = {dy[i].x, dy[i].y, dy[i].z, dy[i].w}, x[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        dot2 = fma2(mul2(bf16x2_to_f32x2(d[j]), pack2(g[i][2 * j], g[i][2 * j + 1])), bf16x2_to_f32x2(x[j]), dot2);
+    }
+    float d0, d1;
+    unpack2(dot2, d0, d1);
+    const float dot = block_sum(d0 + d1, slot[turn]);
+    if (tid == 0 && row != blockIdx.x) {     // the row before this one is done with
+      const int64_t next = row + (int64_t)(stages - 1) * gridDim.x;
+      if (next < a.rows) fetch(next, last);
+    }
+    const float c = -rstd * rstd * (dot * inv);
+    const f32x2_t c2 = pack2(c, c), r2 = pack2(rstd, rstd);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = i * blockDim.x + tid;
+      if (v < nvec) {
+        uint4 rs = make_uint4(0, 0, 0, 0);
+        if (a.dres != nullptr) rs = *reinterpret_cast<const uint4*>(p + 2 * row_bytes + v * 16);
+        const uint32_t d[4] = {dy[i].x, dy[i].y, dy[i].z, dy[i].w}, x[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+        const uint32_t r[4] = {rs.x, rs.y, rs.z, rs.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x2_t dv = bf16x2_to_f32x2(d[j]), xv = bf16x2_to_f32x2(x[j]), gv = pack2(g[i][2 * j], g[i][2 * j + 1]);
+          o[j] = f32x2_to_bf16x2(fma2(r2, fma2(dv, gv, mul2(xv, c2)), bf16x2_to_f32x2(r[j])));
+          const f32x2_t sum = fma2(dv, mul2(xv, r2), pack2(acc[i][2 * j], acc[i][2 * j + 1]));
+          unpack2(sum, acc[i][2 * j], acc[i][2 * j + 1]);
+        }
+        *reinterpret_cast<uint4*>(a.dx + row * a.cols + (int64_t)v * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    last = s;
+    if (++s == stages) { s = 0; ph ^= 1; }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = i * blockDim.x + tid;
+    if (v >= nvec) continue;
+    float4* q = reinterpret_cast<float4*>(a.partial + (int64_t)blockIdx.x * a.cols + (int64_t)v * 8);
+    q[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    q[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+  }
+  pdl_trigger();
+}
+
+// dgamma[k] = sum of `parts` partial rows, in a fixed order. 32 columns per CTA, one row group per warp.
+constexpr int RN_SUM_GROUPS = 16;
+__global__ void __launch_bounds__(32 * RN_SUM_GROUPS) rmsnorm_dgamma_kernel(const float* partial, int parts, int64_t cols,
+                                                                           float* dgamma) {
+  __shared__ float sum[RN_SUM_GROUPS][32];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + lane;
   pdl_trigger();
   pdl_wait();
   float v = 0.0f;
   if (col < cols)
-    for (int p = grp; p < parts; p += 8) v += partial[(int64_t)p * cols + col];
+#pragma unroll 4
+    for (int p = grp; p < parts; p += RN_SUM_GROUPS) v += partial[(int64_t)p * cols + col];
   sum[grp][lane] = v;
   __syncthreads();
   if (grp == 0 && col < cols) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += sum[i][lane];
+    for (int i = 1; i < RN_SUM_GROUPS; ++i) v += sum[i][lane];
     dgamma[col] = v;
   }
 }
@@ -559,11 +694,33 @@ __global__ void __launch_bounds__(256) rmsnorm_dgamma_kernel(const float* partia
 // Threads per row for V vectors per thread (a multiple of 64: whole groups of four segments).
 static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / V + 63) / 64 * 64); }
 
-static int rn_grad_ctas(int64_t rows) {
-  const int64_t most = 2 * (int64_t)mx_sm_count();
+// CTAs per SM that share its memory for their rings, one vector of 8 columns per thread. Two CTAs of 512 threads on 4096 columns and one of 1024 on 8192: with two vectors per thread (two CTAs of
+// 512) the gradient of 8192 x 8192 took 119 us instead of 85.
+static int rn_ring_ctas_per_sm(int64_t cols) { return cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1; }
+static int rn_ring_stages(int64_t cols, int64_t stage) {
+  const int64_t n = RN_RING_BYTES / rn_ring_ctas_per_sm(cols) / stage;
+  return (int)(n < RN_RING_STAGES ? n : RN_RING_STAGES);
+}
+static int rn_grad_ctas(int64_t rows, int64_t cols) {
+  const int64_t most = (int64_t)rn_ring_ctas_per_sm(cols) * mx_sm_count();
   return (int)(rows < most ? rows : most);
 }
-
+template <int V, int kMaxThreads, int kMinCtas>
+static int launch_grad_ring(RmsNormGradArgs& a, int ctas, cudaStream_t st) {
+  auto kern = rmsnorm_grad_ring_kernel<V, kMaxThreads, kMinCtas>;
+  static bool attr_set[MT_MAX_DEVICES] = {};
+  const int slot = current_device_slot();
+  if (!attr_set[slot]) {
+    MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RN_RING_BYTES));
+    attr_set[slot] = true;
+  }
+  const int64_t stage = a.cols * (a.dres ? 6 : 4);
+  a.stages = rn_ring_stages(a.cols, stage);
+  a.status = device_status_ptr();
+  if (!a.status) return fail(MT_ERR_CUDA, "device status word not reachable");
+  MT_CUDA(launch_pdl(kern, dim3(ctas), dim3(rn_threads(a.cols, V)), (size_t)(a.stages * stage), st, a));
+  return MT_OK;
+}
 static bool row_aligned(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
 
 }  // namespace mt
@@ -603,7 +760,8 @@ extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* r
   if (q_t) return rmsnorm_panel(a, st);
   const dim3 grid((unsigned)(s_swz ? padded : rows));
   // Few rows: one vector per thread, the shortest way through a row. Many rows: four vectors per thread, so that more
-  // rows (and bytes) are in flight per SM: 8192 x 4096 with a residual takes 54 us with one vector, XX with four.
+  // rows (and bytes) are in flight per SM. 8192 x 4096 with one vector / with four / with a ring of rows in shared
+  // memory as in the gradient: h and y 54 / 48 / 53 us, y alone 47 / 26 / 46 us, h, y and codes 65 / 57 / 64 us.
   const bool many = rows >= 4 * mx_sm_count();
   if (cols <= 8192 && !many) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<1, 1024>, grid, dim3(rn_threads(cols, 1)), 0, st, a));
   else if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_rows_kernel<4, 256>, grid, dim3(rn_threads(cols, 4)), 0, st, a));
@@ -613,7 +771,7 @@ extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* r
 
 extern "C" int64_t mt_rmsnorm_backward_workspace(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (int64_t)mt::rn_grad_ctas(rows) * cols * 4;
+  return (int64_t)mt::rn_grad_ctas(rows, cols) * cols * 4;
 }
 
 extern "C" int mt_rmsnorm_backward(const void* dy, int64_t dy_stride, const void* h, int64_t h_stride, const void* gamma,
@@ -645,11 +803,14 @@ extern "C" int mt_rmsnorm_backward(const void* dy, int64_t dy_stride, const void
   a.gamma = gamma; a.gamma_f32 = gamma_dtype == MT_F32; a.rstd = rstd;
   a.rows = rows; a.cols = cols;
   a.dx = static_cast<__nv_bfloat16*>(dx); a.partial = static_cast<float*>(workspace);
-  const int ctas = rn_grad_ctas(rows);
-  if (cols <= 8192) MT_CUDA(launch_pdl(rmsnorm_grad_kernel<1>, dim3(ctas), dim3(rn_threads(cols, 1)), 0, st, a));
-  else if (cols <= 16384) MT_CUDA(launch_pdl(rmsnorm_grad_kernel<2>, dim3(ctas), dim3(rn_threads(cols, 2)), 0, st, a));
-  else MT_CUDA(launch_pdl(rmsnorm_grad_kernel<4>, dim3(ctas), dim3(rn_threads(cols, 4)), 0, st, a));
-  MT_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st,
+  const int ctas = rn_grad_ctas(rows, cols);
+  int rc = MT_OK;
+  if (cols <= 4096) rc = launch_grad_ring<1, 512, 2>(a, ctas, st);
+  else if (cols <= 8192) rc = launch_grad_ring<1, 1024, 1>(a, ctas, st);
+  else if (cols <= RN_RING_MAX_COLS) rc = launch_grad_ring<2, 1024, 1>(a, ctas, st);
+  else MT_CUDA(launch_pdl(rmsnorm_grad_kernel<4>, dim3(ctas), dim3(rn_threads(cols, 4)), 0, st, a));   // two rows do not fit
+  if (rc != MT_OK) return rc;
+  MT_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(32 * RN_SUM_GROUPS), 0, st,
                      static_cast<const float*>(workspace), ctas, cols, dgamma));
   return MT_OK;
 }

@@ -499,3 +499,16 @@ def test_refusals_on_the_gpu():
         with torch.no_grad():
             GatedLinear(64, 64, params_dtype=BF, qlinear_params=MXFP8)(x[:2], inp_meta=norm.output_meta)
     assert K.read_device_status() == 0
+
+
+@pytest.mark.parametrize("rows,cols", [(700, 64), (1021, 2080), (640, 8192), (593, 4096), (600, 16384)])
+def test_norm_of_many_rows(rows, cols):
+    """Rows enough for the persistent kernels, each CTA taking several: same bits as the same rows in small batches."""
+    x, r, gamma = _rand((rows, cols), 1, 2.0), _rand((rows, cols), 2), _rand((cols,), 3) + 1
+    for residual in (r, None):
+        for transpose in (False, True):
+            res = _check_norm(x, gamma, residual, 1e-5, transpose)
+        for a in range(0, rows, 250):
+            part = K.rmsnorm(x[a:a + 250], gamma, 1e-5, residual=None if residual is None else r[a:a + 250], quantize=False)
+            assert torch.equal(part.y, res.y[a:a + 250]) and torch.equal(part.rstd, res.rstd[a:a + 250])
+    assert K.read_device_status() == 0
