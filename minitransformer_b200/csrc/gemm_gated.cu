@@ -23,7 +23,7 @@
 
 #include "gated_act.cuh"
 #include "gemm_common.cuh"
-#include "quantize_common.cuh"
+#include "tile_quant.cuh"
 
 namespace mt {
 
@@ -40,6 +40,7 @@ struct GatedArgs {
   uint8_t *q, *s, *s_swz;
   int64_t s_stride, kc_h;                // kc_h: chunks per 128-row block of s_swz
   int tiles_m, tiles_n, num_tiles;
+  int band;                              // pair kernel: row blocks per band of the tile order
 };
 
 __device__ __forceinline__ float gated_alpha(const GatedArgs& a) {
@@ -174,38 +175,67 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       tc_fence_after();
       const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(qd * 32) << 16);
       uint8_t* chunk = a.s_swz + (int64_t)tile * 512;   // tokens of one 128-row block, blocks 4 tile ..
+      const int M = (int)a.M;
 #pragma unroll 1
-      for (int c = 0; c < BT; c += 32) {
-        if (c >= a.M) break;
+      for (int c = 0; c < M; c += 32) {
         uint32_t g[32], u[32];
         tc_ld_32x32(lane_base + Cfg::TMEM_G + c, g);
         tc_ld_32x32(lane_base + Cfg::TMEM_U + c, u);
         tc_wait_ld();
+        const int n = min(32, M - c);     // (columns beyond the last token hold zeros: their rows of x are not there)
+        if (a.gu != nullptr && f_ok) {
+          __nv_bfloat16* p = a.gu + (int64_t)c * 2 * a.F + f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i < n) {
+              p[0] = __float2bfloat16_rn(alpha * __uint_as_float(g[i]));
+              p[a.F] = __float2bfloat16_rn(alpha * __uint_as_float(u[i]));
+            }
+            p += 2 * a.F;
+          }
+        }
+        // h of 32 tokens, all independent of one another; bf16 bits in the upper half of the word
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const int64_t t = c + i;
-          if (t >= a.M) break;
-          const float gv = alpha * __uint_as_float(g[i]), uv = alpha * __uint_as_float(u[i]);
-          const __nv_bfloat16 hb = __float2bfloat16_rn(gated_act_any(a.act, gv) * uv);
-          const float hv = __bfloat162float(hb);
-          if (f_ok) {
-            if (a.h != nullptr) a.h[t * a.F + f] = hb;
-            if (a.gu != nullptr) {
-              a.gu[t * 2 * a.F + f] = __float2bfloat16_rn(gv);
-              a.gu[t * 2 * a.F + a.F + f] = __float2bfloat16_rn(uv);
-            }
-            am.f = fmaxf(am.f, fabsf(hv));
+          const float h = gated_act_any(a.act, alpha * __uint_as_float(g[i])) * (alpha * __uint_as_float(u[i]));
+          g[i] = f_ok ? static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(h))) << 16 : 0u;
+        }
+        if (a.h != nullptr && f_ok) {
+          __nv_bfloat16* p = a.h + (int64_t)c * a.F + f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i < n) *p = __ushort_as_bfloat16(static_cast<unsigned short>(g[i] >> 16));
+            p += a.F;
           }
-          if (a.q != nullptr) {
-            // bit patterns of non-negative floats order like integers; a NaN is dropped as in mt_quantize_mxfp8
-            const float av = fmaxf(fabsf(hv), 0.0f);
-            const int e = e8m0_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, f_ok ? __float_as_uint(av) : 0u)));
-            if (f_ok) a.q[t * a.F + f] = __nv_cvt_float_to_fp8(hv * exp2_neg(e), __NV_SATFINITE, __NV_E4M3);
-            if (lane == 0) {
-              const uint8_t sb = static_cast<uint8_t>(e + 127);
-              if (f_ok && a.s != nullptr) a.s[t * a.s_stride + kb] = sb;
-              if (a.s_swz != nullptr) chunk[sf_chunk_offset((int)t, kb)] = f_ok ? sb : 0;
-            }
+        }
+        if (a.amax != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < n) am.f = fmaxf(am.f, fabsf(__uint_as_float(g[i])));
+        }
+        if (a.q != nullptr) {
+          // lane i ends up with token i's abs-max over the block (bit patterns of magnitudes order like integers; a
+          // NaN is dropped as in mt_quantize_mxfp8) and computes its scale once
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(__uint_as_float(g[i])), 0.0f)));
+            if (lane == i) top = m;
+          }
+          uint32_t enc;
+          const uint32_t sb = mx_scale(top >> 16, enc);
+          uint8_t* p = a.q + (int64_t)c * a.F + f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float e = __uint_as_float(__shfl_sync(0xffffffffu, enc, i) << 16);
+            if (i < n && f_ok) *p = __nv_cvt_float_to_fp8(__uint_as_float(g[i]) * e, __NV_SATFINITE, __NV_E4M3);
+            p += a.F;
+          }
+          const int t = c + lane;
+          if (t < M) {
+            const bool in = (int64_t)kb * 32 < a.F;
+            if (in && a.s != nullptr) a.s[t * a.s_stride + kb] = static_cast<uint8_t>(sb);
+            if (a.s_swz != nullptr) chunk[sf_chunk_offset(t, kb)] = in ? static_cast<uint8_t>(sb) : 0;
           }
         }
       }
@@ -229,6 +259,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 // ------------------------------------------------------------------------------------------
 // M > 128
 // ------------------------------------------------------------------------------------------
+// 16 row blocks (4096 rows) per band: at 8192 x 4096 x 14336 with both bf16 outputs, bands of 1 / 4 / 8 / 16 / 32 took
+// 474 / 442 / 422 / 412 / 411 us (NVFP4) and 870 / 741 / 715 / 702 / 704 us (MXFP8, whose weight alone fills L2).
+constexpr int GP_BAND = 16;
 constexpr int GP_EPI_WARPS = 8;
 constexpr int GP_THREADS = 64 + 32 * GP_EPI_WARPS;
 
@@ -250,6 +283,15 @@ struct GatedPairCfg {
   static_assert(TMEM_SFB + 8 * CH <= G_TMEM_COLS, "tensor memory over-subscribed");
   static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory over-subscribed");
 };
+
+// Tile order of the pair kernel: bands of row blocks, the row block fastest inside a band. The weight tiles are read
+// once per band and the band's rows of x stay in L2 meanwhile.
+__device__ __forceinline__ void gated_tile(const GatedArgs& a, int tile, int& mb, int& nb) {
+  const int per_band = a.band * a.tiles_n, b = tile / per_band, r = tile - b * per_band;
+  const int rows = min(a.band, a.tiles_m - b * a.band);
+  nb = r / rows;
+  mb = b * a.band + (r - nb * rows);
+}
 
 // 32 features of one row: bf16 h (and bf16 g, u) -> global memory, codes and scale byte.
 template <int kAct>
@@ -362,7 +404,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_THREADS, 1)
       bool alive = true;
       const CUtensorMap* map_w = rank == 0 ? &map_g : &map_u;
       for (int tile = pair; tile < a.num_tiles && alive; tile += num_pairs) {
-        const int mb = tile / a.tiles_n, nb = tile - mb * a.tiles_n;
+        int mb, nb;
+        gated_tile(a, tile, mb, nb);
         const int32_t x_row = mb * 256 + (int)rank * 128, w_row = nb * 128;
         const int32_t sx_chunk = (int32_t)((2 * mb + (int)rank) * a.kc), sw_chunk = (int32_t)(nb * a.kc);
         for (int k = 0; k < num_k; ++k) {
@@ -424,7 +467,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_THREADS, 1)
     uint32_t tile_it = 0;
     AmaxAcc am;
     for (int tile = pair; tile < a.num_tiles; tile += num_pairs, ++tile_it) {
-      const int mb = tile / a.tiles_n, nb = tile - mb * a.tiles_n;
+      int mb, nb;
+      gated_tile(a, tile, mb, nb);
       if (!mbar_wait_bounded(acc_full, tile_it & 1, abort_flag, a.status, DS_ACC_FULL_WAIT)) break;
       tc_fence_after();
       const uint32_t tm = tmem_base + (static_cast<uint32_t>(qd * 32) << 16) + half * 64;
@@ -533,6 +577,7 @@ static int launch_gated(const uint8_t* x, const uint8_t* wg, const uint8_t* wu, 
   if (rc != MT_OK) return rc;
   a.tiles_m = (int)((a.M + 255) / 256);
   a.num_tiles = a.tiles_m * a.tiles_n;
+  a.band = GP_BAND;
   constexpr int ST = kFormat == FMT_NVFP4 ? 5 : 6;
   return a.act == MT_ACT_SILU ? launch_gated_pair<kFormat, ST, MT_ACT_SILU>(m, a, st)
                               : launch_gated_pair<kFormat, ST, MT_ACT_GELU>(m, a, st);

@@ -27,7 +27,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    """Handle of the current stream of the current device (without building a Stream object: a tenth of the time)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _require_cuda(t: torch.Tensor, name: str):
@@ -36,7 +37,8 @@ def _require_cuda(t: torch.Tensor, name: str):
 
 
 def swizzled_scale_bytes(rows: int, k_blocks: int) -> int:
-    return int(_lib.load().mt_swizzled_scale_bytes(rows, k_blocks))
+    """mt_swizzled_scale_bytes: 512-byte chunks of 128 rows x 4 blocks, their count along K a multiple of four."""
+    return (rows + 127) // 128 * ((k_blocks + 15) // 16 * 4) * 512
 
 
 @dataclass
