@@ -31,6 +31,15 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def _empty2(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    """torch.empty((rows, cols)) in two thirds of its host time."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
+def _empty1(n: int, dtype, device) -> torch.Tensor:
+    return torch.empty_strided((n,), (1,), dtype=dtype, device=device)
+
+
 def _require_cuda(t: torch.Tensor, name: str):
     if not t.is_cuda:
         raise _lib.MtError(f"{name} must be a CUDA tensor: these kernels have no CPU path")
@@ -121,7 +130,9 @@ def _out_bytes(into, key: str, shape, device) -> torch.Tensor:
         buf = into[key]
         assert buf.dtype == torch.uint8 and buf.is_contiguous() and buf.numel() >= n and buf.data_ptr() % 16 == 0
         return buf[:n].view(*shape)
-    return torch.empty(shape, dtype=torch.uint8, device=device)
+    if len(shape) == 2:
+        return _empty2(shape[0], shape[1], torch.uint8, device)
+    return _empty1(shape[0], torch.uint8, device)
 
 
 def quantized_shard_bytes(fmt: str, rows: int, cols: int):
@@ -179,13 +190,13 @@ def quantize_mxfp8(x: torch.Tensor, *, return_transpose: bool = True, into=None)
     dev = x.device
     u8 = torch.uint8
     q = _out_bytes(into, "q", (M, K), dev)
-    s = torch.empty((M, K // 32), dtype=u8, device=dev)
+    s = _empty2(M, K // 32, u8, dev)
     s_swz = _out_bytes(into, "s_swz", (swizzled_scale_bytes(M, K // 32),), dev)
     q_t = s_t = s_t_swz = None
     mb = (M + 31) // 32
     if return_transpose:
         q_t = _out_bytes(into, "q_t", (K, M), dev)
-        s_t = torch.empty((K, mb), dtype=u8, device=dev)
+        s_t = _empty2(K, mb, u8, dev)
         s_t_swz = _out_bytes(into, "s_t_swz", (swizzled_scale_bytes(K, mb),), dev)
     _lib.call("mt_quantize_mxfp8", x.data_ptr(), M, K, q.data_ptr(), s.data_ptr(), K // 32, s_swz.data_ptr(),
               _ptr(q_t), _ptr(s_t), mb, _ptr(s_t_swz), _stream())
@@ -231,7 +242,7 @@ def _gemm_out(M, N, out_dtype, out, accumulate, device):
     if out is None:
         if accumulate:
             raise _lib.MtError("accumulate=True needs an output tensor")
-        out = torch.empty((M, N), dtype=out_dtype, device=device)
+        out = _empty2(M, N, out_dtype, device)
     else:
         assert out.shape == (M, N) and out.dtype == out_dtype and out.stride(1) == 1
     return out
@@ -525,9 +536,10 @@ def _on_tensor_device(fn):
 
 
 def _same_device(first, **others):
+    dev = first.device
     for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise _lib.MtError(f"{name} is on {t.device}, expected {first.device}")
+        if t is not None and t.device != dev:
+            raise _lib.MtError(f"{name} is on {t.device}, expected {dev}")
 
 
 def _rows(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
@@ -535,9 +547,10 @@ def _rows(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
     when its own layout is not like that."""
     if t.dtype != torch.bfloat16 or t.dim() != 2:
         raise _lib.MtError(f"{name} must be a 2-D bf16 tensor, got {tuple(t.shape)} {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise _lib.MtError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.numel() and (t.stride(1) != 1 or t.stride(0) < t.shape[1] or t.stride(0) % 8 or t.data_ptr() % 16):
+    pitch, unit = t.stride()
+    if (unit != 1 or pitch < t.shape[1] or pitch % 8 or t.data_ptr() % 16) and t.numel():
         # (clone: a one-row or one-column slice may call itself contiguous and still start off a 16-byte address)
         t = t.clone(memory_format=torch.contiguous_format)
     return t
@@ -545,7 +558,7 @@ def _rows(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
 
 def _row_stride(t: torch.Tensor) -> int:
     """Row stride for the C ABI (that of a single row is of no account and may be anything)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _gamma(weight: torch.Tensor, cols: int) -> torch.Tensor:
@@ -567,13 +580,13 @@ def _amax_scalar(device) -> torch.Tensor:
 def _mxfp8_outputs(rows: int, cols: int, transpose: bool, device) -> Quantized:
     """Buffers for the MXFP8 copies of a [rows, cols] tensor."""
     u8 = torch.uint8
-    c = Quantized(torch.empty((rows, cols), dtype=u8, device=device), torch.empty((rows, cols // 32), dtype=u8, device=device),
-                  torch.empty(swizzled_scale_bytes(rows, cols // 32), dtype=u8, device=device))
+    kb = cols // 32
+    c = Quantized(_empty2(rows, cols, u8, device), _empty2(rows, kb, u8, device), _empty1(swizzled_scale_bytes(rows, kb), u8, device))
     if transpose:
         mb = (rows + 31) // 32
-        c.data_t = torch.empty((cols, rows), dtype=u8, device=device)
-        c.scale_t = torch.empty((cols, mb), dtype=u8, device=device)
-        c.scale_t_swz = torch.empty(swizzled_scale_bytes(cols, mb), dtype=u8, device=device)
+        c.data_t = _empty2(cols, rows, u8, device)
+        c.scale_t = _empty2(cols, mb, u8, device)
+        c.scale_t_swz = _empty1(swizzled_scale_bytes(cols, mb), u8, device)
     return c
 
 
@@ -603,16 +616,16 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residua
     x = _rows(x, "x")
     M, C = x.shape
     if residual is not None:
-        residual = _rows(residual, "residual", (M, C))
+        residual = _rows(residual, "residual", x.shape)
     weight = _gamma(weight, C)
     if not (want_y or quantize):
         raise _lib.MtError("rmsnorm: neither y nor its MXFP8 copies requested")
     dev = x.device
-    h = x if residual is None else torch.empty((M, C), dtype=torch.bfloat16, device=dev)
-    rstd = torch.empty(M, dtype=torch.float32, device=dev)
+    h = x if residual is None else _empty2(M, C, torch.bfloat16, dev)
+    rstd = _empty1(M, torch.float32, dev)
     # rows too long for the kernel that makes both copies: y, then the quantize kernel
     after = quantize and return_transpose and C > _NORM_PANEL_COLS
-    y = torch.empty((M, C), dtype=torch.bfloat16, device=dev) if want_y or after else None
+    y = _empty2(M, C, torch.bfloat16, dev) if want_y or after else None
     amax = _amax_scalar(dev) if want_amax else None
     c = _mxfp8_outputs(M, C, return_transpose, dev) if quantize and not after else _NO_COPIES
     _lib.call("mt_rmsnorm_forward", x.data_ptr(), _row_stride(x), _ptr(residual), 0 if residual is None else _row_stride(residual),
@@ -633,16 +646,17 @@ def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rs
     _same_device(dy, h=h, weight=weight, rstd=rstd, dresidual=dresidual)
     dy = _rows(dy, "dy")
     M, C = dy.shape
-    h = _rows(h, "h", (M, C))
+    h = _rows(h, "h", dy.shape)
     weight = _gamma(weight, C)
     if rstd.dtype != torch.float32 or rstd.shape != (M,) or not rstd.is_contiguous():
         raise _lib.MtError(f"rstd must be a contiguous fp32 tensor of {M} values")
     if dresidual is not None:
-        dresidual = _rows(dresidual, "dresidual", (M, C))
-    dx = torch.empty((M, C), dtype=torch.bfloat16, device=dy.device)
-    dweight = torch.empty(C, dtype=torch.float32, device=dy.device)
+        dresidual = _rows(dresidual, "dresidual", dy.shape)
+    dev = dy.device
+    dx = _empty2(M, C, torch.bfloat16, dev)
+    dweight = _empty1(C, torch.float32, dev)
     n = int(_lib.load().mt_rmsnorm_backward_workspace(M, C))
-    work = torch.empty(n, dtype=torch.uint8, device=dy.device) if n else None
+    work = _empty1(n, torch.uint8, dev) if n else None
     _lib.call("mt_rmsnorm_backward", dy.data_ptr(), _row_stride(dy), h.data_ptr(), _row_stride(h), weight.data_ptr(),
               _out_dtype_code(weight.dtype), rstd.data_ptr(), _ptr(dresidual),
               0 if dresidual is None else _row_stride(dresidual), M, C, dx.data_ptr(), dweight.data_ptr(), _ptr(work), n,
@@ -690,24 +704,21 @@ def _gemm_gated(fmt, qa, sa_swz, amax_a, qb, sb_swz, amax_b, activation, sb_lin,
         if sb_lin is None or sb_lin.shape[0] < 2 * F:
             raise _lib.MtError(f"gated projection: F = {F} is not a multiple of 128, which needs the row-major weight scales (sb_lin)")
         sb_up = swizzle_scales(sb_lin[F:2 * F])
-    dev, u8 = qa.device, torch.uint8
+    dev = qa.device
     r = GatedResult()
     o = _lib.GatedOutputs()
     if want_h:
-        r.h = torch.empty((M, F), dtype=torch.bfloat16, device=dev)
+        r.h = _empty2(M, F, torch.bfloat16, dev)
         o.h = r.h.data_ptr()
     if want_gu:
-        r.gu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dev)
+        r.gu = _empty2(M, 2 * F, torch.bfloat16, dev)
         o.gu = r.gu.data_ptr()
     if want_amax:
         r.amax = _amax_scalar(dev)
         o.amax = r.amax.data_ptr()
     if quantize_h:
-        q = torch.empty((M, F), dtype=u8, device=dev)
-        s = torch.empty((M, F // 32), dtype=u8, device=dev)
-        s_swz = torch.empty(swizzled_scale_bytes(M, F // 32), dtype=u8, device=dev)
-        r.quantized = Quantized(q, s, s_swz)
-        o.q, o.s, o.s_stride, o.s_swz = q.data_ptr(), s.data_ptr(), F // 32, s_swz.data_ptr()
+        c = r.quantized = _mxfp8_outputs(M, F, False, dev)
+        o.q, o.s, o.s_stride, o.s_swz = c.data.data_ptr(), c.scale.data_ptr(), F // 32, c.scale_swz.data_ptr()
     _count(1 if M and F else 0)
     if fmt == "mxfp8":
         _lib.call("mt_gemm_gated_mxfp8", qa.data_ptr(), sa_swz.data_ptr(), qb.data_ptr(), sb_swz.data_ptr(), _ptr(sb_up), M, F, K,
@@ -758,7 +769,7 @@ def gated_backward(dh: torch.Tensor, gu: torch.Tensor, *, activation: str = "sil
     if not (quantize or want_dgu):
         raise _lib.MtError("gated_backward: neither the gradient nor its MXFP8 copies requested")
     amax = _amax_scalar(dh.device) if want_amax else None
-    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dh.device) if want_dgu else None
+    dgu = _empty2(M, 2 * F, torch.bfloat16, dh.device) if want_dgu else None
     c = _mxfp8_outputs(M, 2 * F, True, dh.device) if quantize else _NO_COPIES
     _lib.call("mt_gated_backward", dh.data_ptr(), _row_stride(dh), gu.data_ptr(), M, F, act, _ptr(dgu), _ptr(amax), _ptr(c.data),
               _ptr(c.scale), 2 * F // 32, _ptr(c.scale_swz), _ptr(c.data_t), _ptr(c.scale_t), (M + 31) // 32, _ptr(c.scale_t_swz),
