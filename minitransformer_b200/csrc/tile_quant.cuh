@@ -113,6 +113,26 @@ __device__ __forceinline__ void mx_store_bytes(uint8_t* dst, uint2 v, int n) {
   }
 }
 
+// Eight consecutive bytes per lane, the four lanes of a column making a run of 32 that starts anywhere: as aligned
+// words, each taking the bytes it lacks from the lane before; the run's first and last bytes one by one.
+__device__ __forceinline__ void mx_store_run(uint8_t* dst, uint2 v, bool ok) {
+  const int rg = (threadIdx.x & 31) >> 3;
+  const uint32_t a = reinterpret_cast<uintptr_t>(dst) & 3;
+  const uint32_t before = __shfl_up_sync(0xffffffffu, v.y, 8);
+  if (!ok) return;
+  uint32_t* word = reinterpret_cast<uint32_t*>(dst - a);
+  if (a == 0 || rg > 0) word[0] = __funnelshift_l(before, v.x, 8 * a);
+  word[1] = __funnelshift_l(v.x, v.y, 8 * a);
+  if (a != 0 && (rg == 0 || rg == 3)) {
+    const uint32_t n = rg == 0 ? 4 - a : a;
+    uint8_t* p = rg == 0 ? dst : dst + 8 - a;
+    uint32_t b = rg == 0 ? v.x : v.y >> (8 * (4 - a));
+#pragma unroll
+    for (uint32_t k = 0; k < 3; ++k, b >>= 8)
+      if (k < n) p[k] = static_cast<uint8_t>(b);
+  }
+}
+
 // Codes of the tile -> global memory. row0 / col0: its first row and column (multiples of 32). Columns from
 // `limit` on are not stored; rows beyond o.rows hold zeros. A column block is whole or absent (limit % 32 == 0).
 // The abs-max of a block is reduced over its four lanes so that every exchange halves the number of rows (or
@@ -200,6 +220,10 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
       if (nrow > 0) *reinterpret_cast<uint2*>(dst) = lo;
       dst += o.rows;
       if (nrow > 0) *reinterpret_cast<uint2*>(dst) = hi;
+    } else if (row0 + 32 <= o.rows) {
+      mx_store_run(dst, lo, col_ok);
+      dst += o.rows;
+      mx_store_run(dst, hi, col_ok);
     } else {
       mx_store_bytes(dst, lo, nrow);
       dst += o.rows;
