@@ -284,6 +284,13 @@ struct GatedPairCfg {
   static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory over-subscribed");
 };
 
+// Hands tensor memory back to the issuer in the leader CTA. Relaxed: the accumulator is in registers (tcgen05.wait::ld
+// has returned), and a release would wait for this lane's global stores of the tile before as well (8192 x 4096 x
+// 14336, NVFP4: 412 -> 392 us with the saved projections, 367 -> 342 us without).
+__device__ __forceinline__ void arrive_acc_empty(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Tile order of the pair kernel: bands of row blocks, the row block fastest inside a band. The weight tiles are read
 // once per band and the band's rows of x stay in L2 meanwhile.
 __device__ __forceinline__ void gated_tile(const GatedArgs& a, int tile, int& mb, int& nb) {
@@ -482,7 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_THREADS, 1)
       tc_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty_leader);
+      if (lane == 0) arrive_acc_empty(acc_empty_leader);
       const int64_t row = (int64_t)mb * 256 + rank * 128 + qd * 32 + lane;
       const int64_t f = (int64_t)nb * 128 + half * 64;
 #pragma unroll
