@@ -23,7 +23,7 @@ struct GatedGradArgs {
 // while the warp quantizes and stores. Scale bytes are collected in shared memory and leave as words.
 constexpr int GG_SMEM = 8 * 3 * MX_TILE_BYTES + 128;
 
-template <int kAct>
+template <int kAct, bool kRagged>
 __global__ void __launch_bounds__(256, 2)
     gated_grad_kernel(const __grid_constant__ CUtensorMap map_dh, const __grid_constant__ CUtensorMap map_gu, const GatedGradArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(256, 2)
   if (o.q == nullptr) continue;
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    const MxTileScales sc = p ? mx_tile_store(o, wu, row0, a.F + c0, 2 * a.F) : mx_tile_store(o, wg, row0, c0, a.F);
+    const MxTileScales sc = p ? mx_tile_store<kRagged>(o, wu, row0, a.F + c0, 2 * a.F)
+                              : mx_tile_store<kRagged>(o, wg, row0, c0, a.F);
     const int r = wr * 32 + (lane >> 3) * 8 + (lane & 3) * 2, kb = wc * 2 + ((lane & 7) >> 2);
     const int c = wc * 64 + (lane & 7) * 8 + (lane >> 3) * 2;
 #pragma unroll
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(256, 2)
     for (int p = 0; p < 2; ++p) {
       const uint32_t b0 = (uint32_t)((p ? a.F + f0 : f0) >> 5);
       mx_store_scale_word(*reinterpret_cast<const uint32_t*>(s_row[p][t]), n, n == 4 && (b0 & 3) == 0 && row_words,
-                          r < o.rows ? o.s + (uint32_t)(r * (uint32_t)o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
+                          r < o.rows ? o.s + (r * o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
     }
   } else if (o.q_t != nullptr && f0 + t < a.F) {
     const uint32_t b0 = (uint32_t)(m0 >> 5);
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(256, 2)
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const uint32_t c = (uint32_t)((p ? a.F : 0) + f0) + t, word = *reinterpret_cast<const uint32_t*>(s_col[p][t]);
-      mx_store_scale_word(word, n, n == 4 && col_words, o.s_t + (uint32_t)(c * (uint32_t)o.s_t_stride + b0), nullptr, c, b0, 0);
+      mx_store_scale_word(word, n, n == 4 && col_words, o.s_t + (c * o.s_t_stride + b0), nullptr, c, b0, 0);
       // (token blocks without a row: zeros)
       if (o.s_t_swz != nullptr) *reinterpret_cast<uint32_t*>(o.s_t_swz + mx_swz_offset(c, b0, (uint32_t)o.kc_col)) = word;
     }
@@ -148,16 +149,16 @@ __global__ void __launch_bounds__(256, 2)
   pdl_trigger();
 }
 
-template <int kAct>
+template <int kAct, bool kRagged>
 static int launch_gated_grad(const CUtensorMap& mdh, const CUtensorMap& mgu, const GatedGradArgs& a, cudaStream_t st) {
   static bool attr_set[MT_MAX_DEVICES] = {};
   const int slot = current_device_slot();
   if (!attr_set[slot]) {
-    MT_CUDA(cudaFuncSetAttribute(gated_grad_kernel<kAct>, cudaFuncAttributeMaxDynamicSharedMemorySize, GG_SMEM));
+    MT_CUDA(cudaFuncSetAttribute(gated_grad_kernel<kAct, kRagged>, cudaFuncAttributeMaxDynamicSharedMemorySize, GG_SMEM));
     attr_set[slot] = true;
   }
   const int grid = a.tiles < 2 * mx_sm_count() ? a.tiles : 2 * mx_sm_count();
-  MT_CUDA(launch_pdl(gated_grad_kernel<kAct>, dim3(grid), dim3(256), (size_t)GG_SMEM, st, mdh, mgu, a));
+  MT_CUDA(launch_pdl(gated_grad_kernel<kAct, kRagged>, dim3(grid), dim3(256), (size_t)GG_SMEM, st, mdh, mgu, a));
   return MT_OK;
 }
 
@@ -194,5 +195,8 @@ extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, const void* 
   if (rc == MT_OK) rc = mx_tile_map(&mgu, gu, rows, 2 * F, 2 * F);
   if (rc != MT_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return activation == MT_ACT_SILU ? launch_gated_grad<MT_ACT_SILU>(mdh, mgu, a, st) : launch_gated_grad<MT_ACT_GELU>(mdh, mgu, a, st);
+  const bool ragged = rows % 8 != 0;
+  if (activation == MT_ACT_SILU)
+    return ragged ? launch_gated_grad<MT_ACT_SILU, true>(mdh, mgu, a, st) : launch_gated_grad<MT_ACT_SILU, false>(mdh, mgu, a, st);
+  return ragged ? launch_gated_grad<MT_ACT_GELU, true>(mdh, mgu, a, st) : launch_gated_grad<MT_ACT_GELU, false>(mdh, mgu, a, st);
 }

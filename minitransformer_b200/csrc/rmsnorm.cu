@@ -31,9 +31,10 @@ struct RmsNormArgs {
   MxTileOut out;
 };
 
-// Order in which both forward kernels add the squares of a row, so that a row's result does not
-// depend on which of them ran: of eight columns the even and the odd ones in turn; the eight such sums of a 64-column segment by a
-// tree over lanes 4, 2, 1 apart; the eight segments of a 512-column group in turn; the groups in turn.
+// Order in which both forward kernels add the squares of a row, so that a row's result does not depend
+// on which of them ran: of eight columns the even and the odd ones in turn; the eight such sums of a
+// 64-column segment by a tree over lanes 4, 2, 1 apart; the eight segments of a 512-column group in
+// turn; the groups in turn.
 __device__ __forceinline__ float sum_squares8(const uint4& w) {
   f32x2_t v = bf16x2_to_f32x2(w.x), s = mul2(v, v);
   v = bf16x2_to_f32x2(w.y); s = fma2(v, v, s);
@@ -239,7 +240,7 @@ __device__ __forceinline__ void cluster_data_wait(uint64_t* bar, uint32_t parity
   }
 }
 
-template <int kMaxThreads, int kMinCtas>
+template <int kMaxThreads, int kMinCtas, bool kRagged>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
     rmsnorm_panel_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_r, const RmsNormArgs a) {
   constexpr int WARPS = kMaxThreads / 32;
@@ -374,17 +375,16 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
         const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(absmax2_to_float(am)));
         if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
       }
-      const MxTileScales sc = mx_tile_store(o, yw, row0, col0, a.cols);
+      const MxTileScales sc = mx_tile_store<kRagged>(o, yw, row0, col0, a.cols);
       const uint32_t f0 = (uint32_t)col0 + cg * 8 + rg * 2;    // two adjacent features: both inside or both outside
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         s_row[rg * 8 + (lane & 3) * 2 + j][warp * 2 + (cg >> 2)] = static_cast<uint8_t>(sc.row[j]);
       if (f0 < a.cols) {
-        const uint32_t stride = (uint32_t)o.s_t_stride;
         if (row0 < o.rows) {
-          uint8_t* lin = o.s_t + (f0 * stride + panel);
+          uint8_t* lin = o.s_t + (f0 * o.s_t_stride + panel);
           lin[0] = static_cast<uint8_t>(sc.col[0]);
-          lin[stride] = static_cast<uint8_t>(sc.col[1]);
+          lin[o.s_t_stride] = static_cast<uint8_t>(sc.col[1]);
         }
         if (o.s_t_swz != nullptr) {
           uint8_t* swz = o.s_t_swz + mx_swz_offset(f0, panel, (uint32_t)o.kc_col);
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
       const int n = min(min(4, warps * 2 - warp * 4), (int)(a.cols >> 5) - (int)b0);
       if (n > 0)
         mx_store_scale_word(*reinterpret_cast<const uint32_t*>(&s_row[lane][warp * 4]), n, n == 4 && row_words,
-                            live ? o.s + (uint32_t)(r * (uint32_t)o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
+                            live ? o.s + (r * o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
     }
     if (pad_cols) {
       mx_pad_row_scales(o, row0, 32, tid, blockDim.x);
@@ -422,13 +422,13 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
 
 // 512 columns (8 warps) per CTA and up to 8 CTAs per panel; longer rows take 16 warps per CTA. Groups of 512 columns
 // never straddle two CTAs.
-template <int kMaxThreads, int kMinCtas>
+template <int kMaxThreads, int kMinCtas, bool kRagged>
 static int launch_rmsnorm_panel(RmsNormArgs& a, int warps, int ranks, cudaStream_t st) {
   CUtensorMap mx, mr;
   int rc = mx_tile_map(&mx, a.x, a.rows, a.cols, a.x_stride);
   if (rc == MT_OK) rc = a.r ? mx_tile_map(&mr, a.r, a.rows, a.cols, a.r_stride) : (mr = mx, MT_OK);
   if (rc != MT_OK) return rc;
-  auto kern = rmsnorm_panel_kernel<kMaxThreads, kMinCtas>;
+  auto kern = rmsnorm_panel_kernel<kMaxThreads, kMinCtas, kRagged>;
   const size_t smem = (size_t)warps * 2 * MX_TILE_BYTES + 128;
   static int max_clusters_dev[MT_MAX_DEVICES][9] = {};   // by cluster size, for the full number of warps
   int& max_clusters = max_clusters_dev[current_device_slot()][ranks];
@@ -462,12 +462,13 @@ static int launch_rmsnorm_panel(RmsNormArgs& a, int warps, int ranks, cudaStream
   return MT_OK;
 }
 
+template <bool kRagged>
 static int rmsnorm_panel(RmsNormArgs& a, cudaStream_t st) {
   a.status = device_status_ptr();
   if (!a.status) return fail(MT_ERR_CUDA, "device status word not reachable");
-  if (a.cols <= 512) return launch_rmsnorm_panel<256, 2>(a, (int)((a.cols + 63) / 64), 1, st);
-  if (a.cols <= 4096) return launch_rmsnorm_panel<256, 2>(a, 8, (int)((a.cols + 511) / 512), st);
-  return launch_rmsnorm_panel<512, 1>(a, 16, (int)((a.cols + 1023) / 1024), st);
+  if (a.cols <= 512) return launch_rmsnorm_panel<256, 2, kRagged>(a, (int)((a.cols + 63) / 64), 1, st);
+  if (a.cols <= 4096) return launch_rmsnorm_panel<256, 2, kRagged>(a, 8, (int)((a.cols + 511) / 512), st);
+  return launch_rmsnorm_panel<512, 1, kRagged>(a, 16, (int)((a.cols + 1023) / 1024), st);
 }
 
 // ---- gradient ----
@@ -757,7 +758,7 @@ extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* r
            mx_padded_chunks((rows + 31) / 32)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t padded = (rows + 127) / 128 * 128;
-  if (q_t) return rmsnorm_panel(a, st);
+  if (q_t) return rows % 8 ? rmsnorm_panel<true>(a, st) : rmsnorm_panel<false>(a, st);
   const dim3 grid((unsigned)(s_swz ? padded : rows));
   // Few rows: one vector per thread, the shortest way through a row. Many rows: four vectors per thread, so that more
   // rows (and bytes) are in flight per SM. 8192 x 4096 with one vector / with four / with a ring of rows in shared

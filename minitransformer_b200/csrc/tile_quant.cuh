@@ -68,7 +68,11 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t bits, uint32_t& enc) {
   enc = inf ? (__float_as_uint(exp2_neg(127)) >> 16) : (262u - E) << 7;
   return inf ? 254u : E - 8u;
 }
-__device__ __forceinline__ uint32_t mx_amax_bits(uint32_t m) { return max(m & 0x7FFFu, (m >> 16) & 0x7FFFu); }
+// (absmax2 with zero: a block of nothing but NaN counts as zero, as in mt_quantize_mxfp8)
+__device__ __forceinline__ uint32_t mx_amax_bits(uint32_t m) {
+  m = absmax2(m, 0u);
+  return max(m & 0x7FFFu, (m >> 16) & 0x7FFFu);
+}
 
 // Both halves times a power of two: exact, or so small that E4M3 rounds it to zero.
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -138,6 +142,8 @@ __device__ __forceinline__ void mx_store_run(uint8_t* dst, uint2 v, bool ok) {
 // The abs-max of a block is reduced over its four lanes so that every exchange halves the number of rows (or
 // column pairs) a lane still carries; the lane that ends up with a row computes its scale, and the factors
 // travel back two to a word.
+// kRagged: the row count is not a multiple of 8, so the transposed rows start anywhere.
+template <bool kRagged>
 __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const uint32_t (&w)[8][4], int64_t row0, int64_t col0,
                                                       int64_t limit) {
   const int lane = threadIdx.x & 31, cg = lane & 7, rg = lane >> 3;
@@ -198,13 +204,12 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
   }
   {
     const uint32_t send = (rg & 1) ? m[0] : m[1], keep = (rg & 1) ? m[1] : m[0];
-    m[0] = absmax2(keep, __shfl_xor_sync(0xffffffffu, send, 8));
+    m[0] = absmax2(absmax2(keep, __shfl_xor_sync(0xffffffffu, send, 8)), 0u);
   }
   uint32_t e0, e1;
   sc.col[0] = mx_scale(m[0] & 0x7FFFu, e0);
   sc.col[1] = mx_scale((m[0] >> 16) & 0x7FFFu, e1);
   const uint32_t pair = e0 | (e1 << 16);
-  const bool vec = (o.rows & 7) == 0;
   uint8_t* dst = o.q_t + col * o.rows + row;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -216,7 +221,7 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
                                 e4m3x4_rn(bf16_lo(v[4]), bf16_lo(v[5]), bf16_lo(v[6]), bf16_lo(v[7])));
     const uint2 hi = make_uint2(e4m3x4_rn(bf16_hi(v[0]), bf16_hi(v[1]), bf16_hi(v[2]), bf16_hi(v[3])),
                                 e4m3x4_rn(bf16_hi(v[4]), bf16_hi(v[5]), bf16_hi(v[6]), bf16_hi(v[7])));
-    if (vec) {                       // then a lane has all of its rows or none
+    if (!kRagged) {                  // a lane has all of its rows or none
       if (nrow > 0) *reinterpret_cast<uint2*>(dst) = lo;
       dst += o.rows;
       if (nrow > 0) *reinterpret_cast<uint2*>(dst) = hi;
@@ -234,9 +239,10 @@ __device__ __forceinline__ MxTileScales mx_tile_store(const MxTileOut& o, const 
   return sc;
 }
 
-// Byte offset of the scale of (row, block) in a GEMM layout of kc chunks per 128 rows. 32 bits reach 128 G elements.
-__device__ __forceinline__ uint32_t mx_swz_offset(uint32_t row, uint32_t block, uint32_t kc) {
-  return ((row >> 7) * kc + (block >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)(block & 3));
+// Byte offset of the scale of (row, block) in a GEMM layout of kc chunks per 128 rows. (Its padding lets it pass 32
+// bits where the tensor's own scales would not.)
+__device__ __forceinline__ uint64_t mx_swz_offset(uint32_t row, uint32_t block, uint32_t kc) {
+  return ((uint64_t)(row >> 7) * kc + (block >> 2)) * 512 + sf_chunk_offset((int)(row & 127), (int)(block & 3));
 }
 // The first n scale bytes of `word` (blocks b0 .. of one row) to their places in a row-major row (lin, null: none)
 // and in the GEMM layout (swz, null: none); `whole`: n == 4, b0 % 4 == 0 and lin 4-byte aligned (uniform).

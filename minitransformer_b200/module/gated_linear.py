@@ -46,8 +46,8 @@ class _QuantizedGatedLinear(torch.autograd.Function):
         x = cast_if_needed(x.reshape(-1, x_shape[-1]), activation_dtype)
         M = x.shape[0]
         # The wgrad GEMM contracts over the tokens in whole 32-blocks: a ragged batch is continued with rows of
-        # zeros, which add nothing to any gradient.
-        rows = (M + 31) // 32 * 32 if is_grad_enabled else M
+        # zeros, which add nothing to any gradient (and an empty one becomes 32 of them).
+        rows = max(1, (M + 31) // 32) * 32 if is_grad_enabled else M
         if rows != M:
             x, x_meta = _pad_rows(x, rows), None
         qres_x = op.quantize(x, qlinear_params.x_params, return_transpose=is_grad_enabled, input_meta=x_meta)

@@ -37,7 +37,8 @@ def _same_copies(a, b, what):
         x, y = getattr(a, n), getattr(b, n)
         assert (x is None) == (y is None), (what, n)
         if x is not None:
-            assert x.shape == y.shape and torch.equal(x.view(torch.uint8), y.view(torch.uint8)), (what, n)
+            same = x.shape == y.shape and torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+            assert same, (what, n)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -511,4 +512,72 @@ def test_norm_of_many_rows(rows, cols):
         for a in range(0, rows, 250):
             part = K.rmsnorm(x[a:a + 250], gamma, 1e-5, residual=None if residual is None else r[a:a + 250], quantize=False)
             assert torch.equal(part.y, res.y[a:a + 250]) and torch.equal(part.rstd, res.rstd[a:a + 250])
+    assert K.read_device_status() == 0
+
+
+def test_infinities_and_nan_reach_the_copies_as_in_the_quantize_kernel():
+    """Inputs with infinities and NaN: y and dgu carry them where the formula does, and the copies are the quantize
+    kernel's, finite blocks untouched."""
+    x = _rand((64, 256), 1)
+    x[3, 5], x[40, 7] = float("inf"), float("nan")
+    gamma = torch.ones(256, dtype=BF, device="cuda")
+    for transpose in (True, False):
+        r = K.rmsnorm(x, gamma, return_transpose=transpose)
+        bad = ~torch.isfinite(r.y).all(1)
+        assert bad[3] and bad[40] and int(bad.sum()) == 2
+        _same_copies(r.quantized, K.quantize_mxfp8(r.y, return_transpose=transpose), "inf")
+    gu, dh = _rand((64, 128), 2), _rand((64, 64), 3)
+    gu[1, 64 + 3], dh[33, 9] = float("inf"), float("-inf")
+    r = K.gated_backward(dh, gu, want_dgu=True)
+    assert bool(torch.isinf(r.dgu[1, 3])) and bool(torch.isinf(r.dgu[33, 64 + 9])) and int((~torch.isfinite(r.dgu)).sum()) == 3
+    _same_copies(r.quantized, K.quantize_mxfp8(r.dgu), "inf")
+
+
+def test_gated_linear_without_tokens_and_under_autocast():
+    lin = GatedLinear(64, 96, params_dtype=BF, qlinear_params=MXFP8)
+    x = torch.empty(0, 64, dtype=BF, device="cuda", requires_grad=True)
+    h = lin(x)
+    h.sum().backward()
+    assert h.shape == (0, 96) and x.grad.shape == (0, 64) and not bool(lin.weight.grad.any())
+    master = GatedLinear(64, 96, params_dtype=torch.float32, qlinear_params=MXFP8)
+    with torch.no_grad():
+        master.weight.copy_(lin.weight)
+    x = _rand((48, 64), 1, dtype=torch.float32).requires_grad_()
+    with torch.autocast("cuda", dtype=BF):
+        h = master(x)
+    h.backward(_rand((48, 96), 2))
+    xb = x.detach().to(BF).requires_grad_()
+    lin.weight.grad = None
+    hb = lin(xb)
+    hb.backward(_rand((48, 96), 2))
+    assert torch.equal(h, hb) and x.grad.dtype == torch.float32 and master.weight.grad.dtype == torch.float32
+    assert torch.equal(x.grad, xb.grad.float()) and torch.equal(master.weight.grad.to(BF), lin.weight.grad)
+    with pytest.raises(_lib.MtError, match="bf16"):
+        with torch.autocast("cuda", dtype=torch.float16):
+            master(x)
+
+
+def test_results_do_not_depend_on_what_ran_before():
+    """Kernels that start early wait for the one before them: chains of dependent calls, many times, same bits."""
+    x, r, gamma = _rand((300, 512), 1), _rand((300, 512), 2), _rand((512,), 3) + 1
+    w, dh = _rand((768, 512), 4, 0.05), _rand((300, 384), 5, 1e-2)
+    qw = K.quantize_mxfp8(w)
+
+    def chain():
+        n = K.rmsnorm(x, gamma, residual=r)
+        g = K.gemm_gated_mxfp8(n.quantized.data, n.quantized.scale_swz, qw.data, qw.scale_swz, want_gu=True, quantize_h=True)
+        b = K.gated_backward(dh, g.gu)
+        d = K.gemm_mxfp8(b.quantized.data, b.quantized.scale_swz, qw.data_t, qw.scale_t_swz)
+        dx, dg = K.rmsnorm_backward(d, n.h, gamma, n.rstd, dresidual=n.h)
+        return [n.y, g.h, g.quantized.data, b.quantized.data_t, dx, dg]
+
+    first = chain()
+    for _ in range(30):
+        again = chain()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    before = K.set_launch_overlap(False)
+    try:
+        assert all(torch.equal(a, b) for a, b in zip(first, chain()))
+    finally:
+        K.set_launch_overlap(before)
     assert K.read_device_status() == 0

@@ -1,13 +1,19 @@
 """CPU checks of the norm and gated entry points: refusals before anything reaches a GPU, and the device guard."""
 import ctypes
+import os
+import socket
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from minitransformer_b200 import _lib, kernels
 from minitransformer_b200.module import config
 from minitransformer_b200.module.gated_linear import GatedLinear, gated_linear
+from minitransformer_b200.module.linear import Linear
 from minitransformer_b200.module.rmsnorm import RMSNorm
+from minitransformer_b200.ops import quantization as Q
 
 MXFP8 = config.get_qlinear_params_from_predefined(config.QuantizeRecipe.MXFP8_SUB_CHANNEL)
 
@@ -182,3 +188,89 @@ def test_non_quantized_gated_linear_has_gradients():
     for act in ("silu", "gelu"):
         x, w = torch.randn(3, 32, dtype=torch.float64, requires_grad=True), torch.randn(64, 32, dtype=torch.float64, requires_grad=True)
         assert torch.autograd.gradcheck(lambda a, b: gated_linear(a, b, activation=act, qlinear_params=plain), (x, w))
+
+
+class _ExactOp(Q.QuantizeOpBase):
+    """Test double for the kernels: 'codes' are the values themselves in fp32, products are exact."""
+    supports_allgather = False
+
+    def quantize(self, x, qparams, return_transpose=False, reduce_amax=False, tp_group=None, input_meta=None):
+        x = x.reshape(-1, x.shape[-1]).float().contiguous()
+        one = torch.ones(1, 1)
+        return Q.QuantizeResult(x, one, x.t().contiguous() if return_transpose else None, one if return_transpose else None)
+
+    def qgemm(self, qx, qw, m_params, out_dtype, sx, sw, bias=None, out=None, accumulate=False, global_amax_qx=None,
+              global_amax_qw=None, qparams_x=None, qparams_w=None):
+        return (qx @ qw.t()).to(out_dtype)
+
+    def gated_qgemm(self, qx, qw, sx, sw, activation, global_amax_qx=None, global_amax_qw=None, want_h=True, want_gu=False,
+                    quantize_h=False, want_amax=False):
+        gu = qx @ qw.t()
+        g, u = gu.chunk(2, -1)
+        return kernels.GatedResult((torch.nn.functional.silu(g) * u).to(torch.bfloat16), gu.to(torch.bfloat16) if want_gu else None)
+
+    def gated_backward(self, dh, gu, qparams, activation):
+        g, u = gu.float().chunk(2, -1)
+        s = torch.sigmoid(g)
+        dgu = torch.cat([dh.float() * u * s * (1 + g * (1 - s)), dh.float() * g * s], -1)
+        return self.quantize(dgu, qparams, return_transpose=True)
+
+
+def _column_parallel_worker(rank, world, port, result):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        torch.manual_seed(0)
+        bf = torch.bfloat16
+        T, H, F = 40, 32, 128                          # 40 tokens: continued with zeros to 64
+        x, dy = torch.randn(T, H).to(bf), torch.randn(T, H).to(bf)
+        wg, wu, w2 = (torch.randn(*s).mul(0.2).to(bf) for s in ((F, H), (F, H), (H, F)))
+        p = config.QLinearParams(quantize=True, quantize_op=_ExactOp())
+        kw = dict(params_dtype=bf, device="cpu", qlinear_params=p, tp_group=dist.group.WORLD)
+        fc1 = GatedLinear(H, F, parallel_mode="column", **kw)
+        fc2 = Linear(F, H, parallel_mode="row", bias=False, **kw)
+        assert fc1.weight.shape == (2 * F // world, H) and fc1.weight.tensor_model_parallel and fc1.weight.partition_dim == 0
+        with torch.no_grad():
+            fc1.weight.copy_(torch.cat([wg.chunk(world, 0)[rank], wu.chunk(world, 0)[rank]]))
+            fc2.weight.copy_(w2.chunk(world, 1)[rank])
+        xs = x.clone().requires_grad_()
+        y = fc2(fc1(xs))
+        y.backward(dy)
+        X, G, U, W = (t.double().requires_grad_() for t in (x, wg, wu, w2))
+        ref = (torch.nn.functional.silu(X @ G.t()) * (X @ U.t())) @ W.t()
+        ref.backward(dy.double())
+        rel = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+        tol = 4 * 2.0 ** -8      # at most four roundings to bf16 on the way to any of these
+        grad1 = torch.cat([G.grad.chunk(world, 0)[rank], U.grad.chunk(world, 0)[rank]])
+        errs = [rel(y, ref), rel(xs.grad, X.grad), rel(fc1.weight.grad, grad1), rel(fc2.weight.grad, W.grad.chunk(world, 1)[rank])]
+        result[rank] = errs if max(errs) > tol else True
+    finally:
+        dist.destroy_process_group()
+
+
+def test_column_parallel_gated_linear_on_two_ranks():
+    """Each rank holds [gate shard; up shard]; dgrad is summed over the ranks."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    with mp.get_context("spawn").Manager() as m:
+        result = m.dict()
+        mp.spawn(_column_parallel_worker, args=(2, port, result), nprocs=2, join=True)
+        assert dict(result) == {0: True, 1: True}, dict(result)
+
+
+def test_mx_scale_rule_on_every_bf16_magnitude():
+    """The scale rule of the register quantizer (integer arithmetic on bf16 bits), restated, against its definition."""
+    import math
+    from fractions import Fraction
+    import numpy as np
+    for bits in range(0x7F80):
+        E = max((bits + 0x1F) >> 7, 8)
+        value = Fraction(float(np.array([bits << 16], dtype=np.uint32).view(np.float32)[0]))
+        e = -127
+        if value:
+            e = math.ceil(math.log2(value / 448)) - 2
+            while Fraction(2) ** e < value / 448:
+                e += 1
+            e = max(e, -127)
+        assert E - 8 == e + 127, hex(bits)
