@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
   __shared__ __align__(16) uint8_t s_rows[2][2][128][4], s_cols[2][2][128][4];   // [turn][dg, du][row / feature][block]
-  __shared__ uint64_t bars[8];
+  __shared__ uint64_t bars[8], empty[8];
   __shared__ int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wr = warp & 3, wc = warp >> 2;
@@ -37,7 +37,10 @@ __global__ void __launch_bounds__(256, 2)
   const MxTileOut& o = a.out;
   const bool row_words = mx_word_aligned(o.s, o.s_stride), col_words = mx_word_aligned(o.s_t, o.s_t_stride);
   if (tid == 0) abort_flag = 0;
-  if (lane == 0) mbar_init(&bars[warp], 1);
+  if (lane == 0) {
+    mbar_init(&bars[warp], 1);
+    mbar_init(&empty[warp], 32);
+  }
   mbar_fence_init();
   __syncthreads();
   pdl_wait();
@@ -73,7 +76,7 @@ __global__ void __launch_bounds__(256, 2)
       wg[i][j] = f32x2_to_bf16x2(mul2(mul2(d2, bf16x2_to_f32x2(u[j])), grad));
     }
   }
-  __syncwarp();
+  mx_release_tile(&empty[warp], ph, &abort_flag, a.status);
   if (lane == 0 && tile + (int)gridDim.x < a.tiles) fetch(tile + gridDim.x);
   if (a.dgu != nullptr) {
     const int64_t row = row0 + (lane >> 3) * 8, f = c0 + (lane & 7) * 8;

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
   __shared__ float seg[WARPS][32];                         // this CTA's segments
   __shared__ float grp[2][RN_PANEL_MAX_COLS / 512][32];    // the panel's groups; panels alternate
   __shared__ __align__(16) uint8_t s_row[32][WARPS * 2];
-  __shared__ uint64_t bars[WARPS], xbar[2];
+  __shared__ uint64_t bars[WARPS], empty[WARPS], xbar[2];
   __shared__ int abort_flag;
   const MxTileOut& o = a.out;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
@@ -266,7 +266,10 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
     mbar_init(&xbar[0], 1);
     mbar_init(&xbar[1], 1);
   }
-  if (lane == 0) mbar_init(&bars[warp], 1);
+  if (lane == 0) {
+    mbar_init(&bars[warp], 1);
+    mbar_init(&empty[warp], 32);
+  }
   mbar_fence_init();
   __syncthreads();
   if (ranks > 1) {   // every CTA's barriers exist before anything is sent to it
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas)
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = add_bf16x8(w[i], mx_tile_row(buf + MX_TILE_BYTES, i));
       }
-      __syncwarp();
+      mx_release_tile(&empty[warp], turn & 1, &abort_flag, a.status);
       if (lane == 0 && panel + clusters < panels) fetch(panel + clusters);
     } else {
 #pragma unroll
@@ -630,6 +633,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) rmsnorm_grad_ring_kerne
     }
     float d0, d1;
     unpack2(dot2, d0, d1);
+    fence_proxy_async_smem();                // this thread's reads of the row before come ahead of the copies into its stage
     const float dot = block_sum(d0 + d1, slot[turn]);
     if (tid == 0 && row != blockIdx.x) {     // the row before this one is done with
       const int64_t next = row + (int64_t)(stages - 1) * gridDim.x;

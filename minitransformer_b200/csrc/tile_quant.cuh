@@ -100,7 +100,22 @@ struct MxTileScales {
 // A warp's 32 x 64 bf16 tile as TMA leaves it (rows of 128 bytes): this lane's 16 bytes of row i.
 __device__ __forceinline__ uint4 mx_tile_row(const uint8_t* tile, int i) {
   const int lane = threadIdx.x & 31;
-  return *reinterpret_cast<const uint4*>(tile + ((lane >> 3) * 8 + i) * 128 + (lane & 7) * 16);
+  uint4 v;   // volatile: stays ahead of the buffer's release
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(smem_u32(tile) + ((lane >> 3) * 8 + i) * 128 + (lane & 7) * 16) : "memory");
+  return v;
+}
+
+// Gives a warp's tile buffer back before the next TMA load into it: every lane puts its reads (generic proxy) before the
+// copy engine's writes (async proxy) with the proxy fence and arrives on `empty` (32 arrivals); lane 0, the one that
+// loads, waits for the phase. A __syncwarp, and the arrivals without the fence, let the engine overtake the
+// last reads: some rows of one in ten to one in two calls came out wrong.
+__device__ __forceinline__ void mx_release_tile(uint64_t* empty, uint32_t parity, volatile int* abort_flag, int* status) {
+  fence_proxy_async_smem();
+  mbar_arrive(empty);
+  if ((threadIdx.x & 31) == 0) mbar_wait_bounded(empty, parity, abort_flag, status, DS_EMPTY_WAIT);
+  __syncwarp();
 }
 
 // Rows of [row, row + 8) below `rows`.

@@ -581,3 +581,52 @@ def test_results_do_not_depend_on_what_ran_before():
     finally:
         K.set_launch_overlap(before)
     assert K.read_device_status() == 0
+
+
+@pytest.mark.parametrize("rows,cols", [(8192, 4096), (15665, 704), (15664, 2080), (6001, 8192)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_of_many_panels_repeated(rows, cols, residual):
+    """Clusters that take several panels one after the other, tiles arriving while the ones before are in use."""
+    x, r, gamma = _rand((rows, cols), 1, 2.0), _rand((rows, cols), 2) if residual else None, _rand((cols,), 3) + 1
+    plain = K.rmsnorm(x, gamma, residual=r, quantize=False)
+    copies = K.quantize_mxfp8(plain.y)
+    for _ in range(12):
+        res = K.rmsnorm(x, gamma, residual=r)
+        assert torch.equal(res.rstd, plain.rstd) and torch.equal(res.y, plain.y) and torch.equal(res.h, plain.h)
+        _same_copies(res.quantized, copies, "panels")
+    assert K.read_device_status() == 0
+
+
+@pytest.mark.parametrize("rows,F", [(8192, 4096), (4099, 1376), (2048, 14336)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_gradient_of_many_tiles_repeated(rows, F, act):
+    gu, dh = _rand((rows, 2 * F), 1, 1.5), _rand((rows, F), 2, 1e-2)
+    dgu = K.gated_backward(dh, gu, activation=act, quantize=False, want_dgu=True).dgu
+    g, u = gu.double().split(F, 1)
+    a, d, s, z = _act64(g, act)
+    D = dh.double()
+    soft, slope = (1 + z.abs()) * 2.0 ** -20, s + (d - s).abs()
+    _within(dgu[:, :F], D * u * d, HALF * (D * u * d).abs() + soft * (D * u).abs() * slope + TINY, "dg")
+    _within(dgu[:, F:], D * a, (HALF + soft) * (D * a).abs() + TINY, "du")
+    del g, u, a, d, s, z, D, soft, slope
+    copies = K.quantize_mxfp8(dgu)
+    for _ in range(12):
+        r = K.gated_backward(dh, gu, activation=act, want_dgu=True)
+        assert torch.equal(r.dgu, dgu)
+        _same_copies(r.quantized, copies, "tiles")
+    assert K.read_device_status() == 0
+
+
+@pytest.mark.parametrize("rows,cols", [(8192, 8192), (9001, 2080), (5000, 704)])
+def test_norm_gradient_of_many_rows_repeated(rows, cols):
+    h, gamma, dy, dres = _rand((rows, cols), 1, 2.0), _rand((cols,), 2) + 1, _rand((rows, cols), 3, 0.1), _rand((rows, cols), 4, 0.1)
+    rstd = K.rmsnorm(h, gamma, quantize=False).rstd
+    first = K.rmsnorm_backward(dy, h, gamma, rstd, dresidual=dres)
+    H, R, A = h.double(), rstd.double()[:, None], dy.double() * gamma.double()
+    want = R * A - R ** 3 * H * (A * H).sum(1, keepdim=True) / cols + dres.double()
+    mag = R * A.abs() + R ** 3 * H.abs() * (A * H).abs().sum(1, keepdim=True) / cols + dres.double().abs()
+    _within(first[0], want, HALF * want.abs() + 60 * 2.0 ** -24 * mag + TINY, "dx")
+    for _ in range(12):
+        again = K.rmsnorm_backward(dy, h, gamma, rstd, dresidual=dres)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    assert K.read_device_status() == 0
