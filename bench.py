@@ -1,7 +1,7 @@
 """Benchmark of the quantized-linear hot path.
 
     python bench.py [--gpus N] [--steps K] [--warmup W] [--impl reference]
-    python bench.py --profile-case gemm|gemm_mxfp8|quant|quant_mxfp8|grouped
+    python bench.py --profile-case gemm|gemm_mxfp8|quant|quant_mxfp8|grouped|norm_gated|block
 
 One step = one forward + backward of the NVFP4 Linear of the reference recipe (Hadamard
 transform on the transposed activation / gradient copies) on synthetic data:
@@ -529,12 +529,14 @@ def tp_parity_check(group, T=2048, H=1024, Fd=4096, recipe="fp4_subchannel_scali
 C5 = dict(layers=8, hidden=4096, heads=32, kv_heads=8, ffn=14336, vocab=32000, seq=4096, micro_batch=2)
 
 
-def build_llama_decoder(torch, dims, params, tp_group=None, peer=True, device="cuda"):
+def build_llama_decoder(torch, dims, params, tp_group=None, peer=True, device="cuda", fused_block=False):
     """Llama-style decoder (RMSNorm, grouped-query attention through torch SDPA, gated SiLU MLP)
     whose linears are the drop-in Linear under `params`. With a tensor-parallel group: Megatron
     layout with sequence parallelism (qkv and the gated fc1 column-parallel with their heads /
     ffn columns sharded, proj and fc2 row-parallel, token-sharded activations between blocks, a
-    vocabulary-parallel head and loss). Input ids [micro_batch, seq]; returns the mean loss."""
+    vocabulary-parallel head and loss). Input ids [micro_batch, seq]; returns the mean loss.
+    fused_block (one GPU): the norms with their residual additions and the gated fc1 are the library's RMSNorm and
+    GatedLinear, which hand their MXFP8 copies to the next layer; same parameters under the same names."""
     import torch.distributed as dist
     from minitransformer_b200.module.linear import Linear
     tp = dist.get_world_size(tp_group) if tp_group is not None else 1
@@ -542,6 +544,7 @@ def build_llama_decoder(torch, dims, params, tp_group=None, peer=True, device="c
     H, heads, kvh, ffn, vocab = dims["hidden"], dims["heads"], dims["kv_heads"], dims["ffn"], dims["vocab"]
     hd = H // heads
     assert heads % tp == 0 and kvh % tp == 0 and ffn % tp == 0 and vocab % tp == 0
+    assert tp == 1 or not fused_block, "the fused block runs without sequence parallelism"
     init = lambda t: torch.nn.init.normal_(t, std=0.02)
 
     def lin(i, o, mode, name):
@@ -581,12 +584,40 @@ def build_llama_decoder(torch, dims, params, tp_group=None, peer=True, device="c
             g, u = self.fc1(self.norm2(x)).chunk(2, dim=-1)
             return x + self.fc2(torch.nn.functional.silu(g) * u)
 
+    def fused_norm():
+        from minitransformer_b200.module.rmsnorm import RMSNorm as FusedRMSNorm
+        norm = FusedRMSNorm(H, eps=1e-5, params_dtype=torch.bfloat16, device=device, qlinear_params=params)
+        norm.emit_quantized = True
+        return norm
+
+    class FusedBlock(torch.nn.Module):
+        """x: residual stream; d: what the layer before adds to it (None in the first block)."""
+        def __init__(self):
+            super().__init__()
+            from minitransformer_b200.module.gated_linear import GatedLinear
+            self.norm1, self.norm2 = fused_norm(), fused_norm()
+            self.qkv = lin(H, (heads + 2 * kvh) * hd, "column", "qkv")
+            self.proj = lin(H, H, "row", "proj")
+            self.fc1 = GatedLinear(H, ffn, params_dtype=torch.bfloat16, device=device, qlinear_params=params, init_method=init)
+            self.fc2 = lin(ffn, H, "row", "fc2")
+
+        def forward(self, x, d, B, S):
+            n, x = (self.norm1(x), x) if d is None else self.norm1(d, x)
+            qkv = self.qkv(n, inp_meta=self.norm1.output_meta)
+            q, k, v = qkv.split([heads * hd, kvh * hd, kvh * hd], dim=-1)
+            q = q.view(B, S, heads, hd).transpose(1, 2)
+            k = k.view(B, S, kvh, hd).transpose(1, 2).repeat_interleave(heads // kvh, 1)
+            v = v.view(B, S, kvh, hd).transpose(1, 2).repeat_interleave(heads // kvh, 1)
+            a = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True)
+            n, x = self.norm2(self.proj(a.transpose(1, 2).reshape(B * S, heads * hd)), x)
+            return x, self.fc2(self.fc1(n, inp_meta=self.norm2.output_meta))
+
     class Decoder(torch.nn.Module):
         def __init__(self):
             super().__init__()
             self.emb = torch.nn.Embedding(vocab, H, dtype=torch.bfloat16, device=device)
-            self.blocks = torch.nn.ModuleList([Block() for _ in range(dims["layers"])])
-            self.norm = RMSNorm()
+            self.blocks = torch.nn.ModuleList([FusedBlock() if fused_block else Block() for _ in range(dims["layers"])])
+            self.norm = fused_norm() if fused_block else RMSNorm()
             self.head = lin(H, vocab, "column", "head")
 
         def forward(self, ids, targets):
@@ -594,9 +625,16 @@ def build_llama_decoder(torch, dims, params, tp_group=None, peer=True, device="c
             x = self.emb(ids).view(B * S, H)
             if tp > 1:
                 x = x.chunk(tp, 0)[rank]
-            for b in self.blocks:
-                x = b(x, B, S)
-            logits = self.head(self.norm(x)).float()                      # [B*S, vocab / tp]
+            if fused_block:
+                d = None
+                for b in self.blocks:
+                    x, d = b(x, d, B, S)
+                n, _ = self.norm(d, x)
+                logits = self.head(n, inp_meta=self.norm.output_meta).float()
+            else:
+                for b in self.blocks:
+                    x = b(x, B, S)
+                logits = self.head(self.norm(x)).float()                  # [B*S, vocab / tp]
             t = targets.view(-1)
             if tp == 1:
                 return torch.nn.functional.cross_entropy(logits, t)
@@ -1177,6 +1215,8 @@ def run_profile_case(what: str) -> None:
       quant        abs-max + NVFP4 cast/transpose (RHT) of 8192x14336
       quant_mxfp8  MXFP8 cast/transpose of 8192x14336
       grouped      MXFP8 GroupedLinear fc1+fc2 fwd+bwd, 128 experts, 2 steps
+      norm_gated   norm forward / gradient, gated GEMMs (one token, a batch of rows) and gated gradient, 3 launches each
+      block        two decoder layers of configuration 5, forward + backward, plain and with the fused block: ms per step
       tp_step      (under torchrun, N ranks) the tensor-parallel MLP step of `--gpus N` under the torch
                    profiler: per-kernel device time of three steps and the timeline of the last one"""
     import torch
@@ -1227,6 +1267,38 @@ def run_profile_case(what: str) -> None:
         for _ in range(2):
             xd = x.detach().requires_grad_(True)
             fc2(fc1(xd, m_splits, is_first_microbatch=True), m_splits, is_first_microbatch=True).backward(dy)
+    elif what == "norm_gated":
+        r = lambda *s: torch.randn(*s, device=dev).to(torch.bfloat16)  # noqa: E731
+        x, res, gamma, dy = r(8192, 4096), r(8192, 4096), r(4096), r(8192, 4096)
+        gu, dh, w = r(4096, 2 * 14336), r(4096, 14336), r(2 * 14336, 4096)
+        qw = K.quantize_mxfp8(w, return_transpose=False)
+        q1, qn = K.quantize_mxfp8(x[:1], return_transpose=False), K.quantize_mxfp8(x[:4096], return_transpose=False)
+        for _ in range(3):
+            n = K.rmsnorm(x, gamma, residual=res)
+            K.rmsnorm(x, gamma, residual=res, return_transpose=False)
+            K.rmsnorm_backward(dy, n.h, gamma, n.rstd, dresidual=res)
+            K.gemm_gated_mxfp8(q1.data, q1.scale_swz, qw.data, qw.scale_swz, want_h=False, quantize_h=True)
+            K.gemm_gated_mxfp8(qn.data, qn.scale_swz, qw.data, qw.scale_swz, want_gu=True)
+            K.gated_backward(dh, gu)
+    elif what == "block":
+        from minitransformer_b200.module import config as mt_config
+        params = mt_config.get_qlinear_params_from_predefined(mt_config.QuantizeRecipe.MXFP8_SUB_CHANNEL)
+        dims = dict(C5, layers=2)
+        ids = torch.randint(0, dims["vocab"], (dims["micro_batch"], dims["seq"]), device=dev)
+        for fused in (False, True):
+            torch.manual_seed(0)
+            model = build_llama_decoder(torch, dims, params, device=dev, fused_block=fused)
+
+            def step():
+                for p_ in model.parameters():
+                    p_.grad = None
+                loss = model(ids, ids.roll(-1, 1))
+                loss.backward()
+                return loss.detach()
+
+            ms = _timed_loop(torch, step, 10, 3)
+            print(f"decoder, {dims['layers']} layers, fused block {fused}: {ms:.3f} ms per step, loss {float(step()):.4f}")
+            del model
     else:
         raise SystemExit(f"unknown case {what!r}")
     torch.cuda.synchronize()

@@ -410,12 +410,13 @@ int mt_gemm_gated_nvfp4(const uint8_t* x, const uint8_t* sx_swz, const float* am
                         const mt_gated_outputs* out, mt_stream_t stream);
 
 /* Gradient of h = act(g) * u: du = bf16(dh * act(g)), dg = bf16(dh * u * act'(g)).
- * dh bf16 [rows, F] (row stride dh_stride), gu bf16 [rows, 2F] = [g | u]; F % 32 == 0.
+ * dh bf16 [dh_rows, F] (row stride dh_stride), gu bf16 [rows, 2F] = [g | u]; F % 32 == 0. dh_rows may be smaller
+ * than rows: the gradient of the remaining rows is zero (a batch continued to whole blocks of tokens).
  * Outputs, dgu or q at least: dgu bf16 [rows, 2F] = [dg | du]; amax (optional): device fp32 scalar, raised
  * to max |dgu| (zeroed by the caller); q, s, s_swz, q_t, s_t, s_t_swz: MXFP8 copies of dgu as
  * mt_quantize_mxfp8 makes them (q_t optional). */
-int mt_gated_backward(const void* dh, int64_t dh_stride, const void* gu, int64_t rows, int64_t F, int activation,
-                      void* dgu, float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz,
+int mt_gated_backward(const void* dh, int64_t dh_stride, int64_t dh_rows, const void* gu, int64_t rows, int64_t F,
+                      int activation, void* dgu, float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz,
                       uint8_t* q_t, uint8_t* s_t, int64_t s_t_stride, uint8_t* s_t_swz, mt_stream_t stream);
 
 /* Reads and clears the device-side status word the kernels raise when a bounded wait

@@ -167,8 +167,8 @@ static int launch_gated_grad(const CUtensorMap& mdh, const CUtensorMap& mgu, con
 
 }  // namespace mt
 
-extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, const void* gu, int64_t rows, int64_t F, int activation,
-                                 void* dgu, float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz, uint8_t* q_t,
+extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, int64_t dh_rows, const void* gu, int64_t rows, int64_t F,
+                                 int activation, void* dgu, float* amax, uint8_t* q, uint8_t* s, int64_t s_stride, uint8_t* s_swz, uint8_t* q_t,
                                  uint8_t* s_t, int64_t s_t_stride, uint8_t* s_t_swz, mt_stream_t stream) {
   using namespace mt;
   const char* name = "mt_gated_backward";
@@ -181,6 +181,7 @@ extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, const void* 
   MT_REQUIRE(dgu || q, "%s: no output requested", name);
   MT_REQUIRE(aligned16(dh) && aligned16(gu) && aligned16(dgu), "%s: pointers must be 16-byte aligned", name);
   MT_REQUIRE(dh_stride >= F && dh_stride % 8 == 0, "%s: dh needs 16-byte aligned rows", name);
+  MT_REQUIRE(dh_rows > 0 && dh_rows <= rows, "%s: dh has %lld rows for %lld of gu", name, (long long)dh_rows, (long long)rows);
   int rc = mx_outputs_ok(name, rows, 2 * F, q, s, s_stride, s_swz, q_t, s_t, s_t_stride, s_t_swz);
   if (rc != MT_OK) return rc;
   GatedGradArgs a{};
@@ -194,7 +195,7 @@ extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, const void* 
   a.status = device_status_ptr();
   if (!a.status) return fail(MT_ERR_CUDA, "device status word not reachable");
   CUtensorMap mdh, mgu;
-  rc = mx_tile_map(&mdh, dh, rows, F, dh_stride);
+  rc = mx_tile_map(&mdh, dh, dh_rows, F, dh_stride);   // (rows beyond its own read as zeros)
   if (rc == MT_OK) rc = mx_tile_map(&mgu, gu, rows, 2 * F, 2 * F);
   if (rc != MT_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

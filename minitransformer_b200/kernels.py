@@ -756,14 +756,17 @@ class GatedGradResult:
 @_on_tensor_device
 def gated_backward(dh: torch.Tensor, gu: torch.Tensor, *, activation: str = "silu", quantize: bool = True,
                    want_dgu: bool = False, want_amax: bool = False) -> GatedGradResult:
-    """From dh [M, F] and the projections gu [M, 2F] = [g | u] (bf16): du = dh act(g), dg = dh u act'(g).
+    """From dh [M, F] and the projections gu [M, 2F] = [g | u] (bf16): du = dh act(g), dg = dh u act'(g). dh may have
+    fewer rows than gu: the gradient of the others is zero.
     quantize: MXFP8 copies of [dg | du], row-wise and transposed, bit for bit those of quantize_mxfp8 of the
     bf16 gradient; want_dgu: the bf16 gradient itself."""
     _same_device(dh, gu=gu)
     act = _activation_code(activation)
-    dh = _rows(dh, "dh")
-    M, F = dh.shape
-    gu = _rows(gu, "gu", (M, 2 * F))
+    dh, gu = _rows(dh, "dh"), _rows(gu, "gu")
+    dh_rows, F = dh.shape
+    M = gu.shape[0]
+    if gu.shape[1] != 2 * F or dh_rows > M or (M and not dh_rows):
+        raise _lib.MtError(f"dh of shape {tuple(dh.shape)} for projections of shape {tuple(gu.shape)}")
     if not gu.is_contiguous():
         gu = gu.contiguous()
     if not (quantize or want_dgu):
@@ -771,10 +774,10 @@ def gated_backward(dh: torch.Tensor, gu: torch.Tensor, *, activation: str = "sil
     amax = _amax_scalar(dh.device) if want_amax else None
     dgu = _empty2(M, 2 * F, torch.bfloat16, dh.device) if want_dgu else None
     c = _mxfp8_outputs(M, 2 * F, True, dh.device) if quantize else _NO_COPIES
-    _lib.call("mt_gated_backward", dh.data_ptr(), _row_stride(dh), gu.data_ptr(), M, F, act, _ptr(dgu), _ptr(amax), _ptr(c.data),
-              _ptr(c.scale), 2 * F // 32, _ptr(c.scale_swz), _ptr(c.data_t), _ptr(c.scale_t), (M + 31) // 32, _ptr(c.scale_t_swz),
-              _stream())
-    _count(1 if dh.numel() else 0)
+    _lib.call("mt_gated_backward", dh.data_ptr(), _row_stride(dh), dh_rows, gu.data_ptr(), M, F, act, _ptr(dgu), _ptr(amax),
+              _ptr(c.data), _ptr(c.scale), 2 * F // 32, _ptr(c.scale_swz), _ptr(c.data_t), _ptr(c.scale_t), (M + 31) // 32,
+              _ptr(c.scale_t_swz), _stream())
+    _count(1 if M and F else 0)
     return GatedGradResult(dgu, c if quantize else None, amax)
 
 

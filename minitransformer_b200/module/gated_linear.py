@@ -36,7 +36,7 @@ class _QuantizedGatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, x_meta, w, weight_qresult_cache, activation, tp_group, tp_size, parallel_mode, qlinear_params,
                 activation_dtype, is_grad_enabled, is_first_microbatch, fuse_wgrad_accumulation, out_meta):
-        """out_meta: None, or (a QuantizeInputMeta that receives what the next layer's quantizer can take over,
+        """weight_qresult_cache: None (nothing kept) or a QuantizeResultCache. out_meta: None, or (a QuantizeInputMeta that receives what the next layer's quantizer can take over,
         whether that is the MXFP8 copy of h)."""
         op = qlinear_params.quantize_op
         assert op is not None and hasattr(op, "gated_qgemm"), "the recipe's backend has no gated projection"
@@ -53,13 +53,15 @@ class _QuantizedGatedLinear(torch.autograd.Function):
         qres_x = op.quantize(x, qlinear_params.x_params, return_transpose=is_grad_enabled, input_meta=x_meta)
 
         # (a cache filled under no_grad holds no transposed copy: refill it before a training pass)
-        usable = weight_qresult_cache.data is not None and not (is_grad_enabled and weight_qresult_cache.data_t is None)
-        keep = bool(getattr(weight_qresult_cache, "keep", False)) and usable
+        cache = weight_qresult_cache
+        usable = cache is not None and cache.data is not None and not (is_grad_enabled and cache.data_t is None)
+        keep = usable and bool(getattr(cache, "keep", False))
         if not keep and (is_first_microbatch or is_first_microbatch is None or not usable):
             qres_w = op.quantize(w, qlinear_params.w_params, return_transpose=is_grad_enabled)
-            weight_qresult_cache.store(qres_w)
+            if cache is not None:
+                cache.store(qres_w)
         else:
-            qres_w = weight_qresult_cache.to_qresult()
+            qres_w = cache.to_qresult()
 
         meta, copy = out_meta if out_meta is not None else (None, False)
         r = op.gated_qgemm(qres_x.data, qres_w.data, qres_x.scale, qres_w.scale, activation,
@@ -88,7 +90,10 @@ class _QuantizedGatedLinear(torch.autograd.Function):
             sw_t._mt_swz = ctx.sw_t_swz
         dh = dh.reshape(-1, dh.shape[-1])
         M, grad_dtype = dh.shape[0], dh.dtype
-        dh = _pad_rows(cast_if_needed(dh, torch.bfloat16), ctx.rows)
+        dh = cast_if_needed(dh, torch.bfloat16)
+        if M == 0:
+            dh = _pad_rows(dh, ctx.rows)
+        # (rows that continue a ragged batch have no gradient: the kernel takes dh without them)
         qres_d = op.gated_backward(dh, gu, p.g_params, ctx.activation)
         dgrad = op.qgemm(qres_d.data, qw_t, p.mm_dgrad, p.mm_dgrad.out_dtype or grad_dtype, qres_d.scale, sw_t, None, None,
                          accumulate=False, global_amax_qx=qres_d.global_amax_row, global_amax_qw=amax_w_col,
@@ -128,7 +133,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, *, activation: str = "si
     if not params.quantize:
         return _non_quantized(x, weight, activation)
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
-    args = (x, inp_meta, weight, quantization.QuantizeResultCache(), activation, None, 1, None, params, x.dtype, grad, None,
+    args = (x, inp_meta, weight, None, activation, None, 1, None, params, x.dtype, grad, None,
             False, None)
     return _QuantizedGatedLinear.apply(*args) if grad else _QuantizedGatedLinear.forward(None, *args)
 

@@ -274,6 +274,12 @@ def test_gated_gradient_matches_formula(rows, F, act):
     _within(r.dgu, want, tol + TINY, "dgu")
     _same_copies(r.quantized, K.quantize_mxfp8(r.dgu), "gradient")
     assert float(r.amax) == float(r.dgu.abs().max().float())
+    if rows > 1:     # dh with fewer rows: as with zeros in the rest
+        n = rows // 2 + 1
+        part = K.gated_backward(dh[:n], gu, activation=act, want_dgu=True)
+        full = K.gated_backward(torch.cat([dh[:n], torch.zeros_like(dh[n:])]), gu, activation=act, want_dgu=True)
+        assert torch.equal(part.dgu, full.dgu) and not bool(part.dgu[n:].any())
+        _same_copies(part.quantized, full.quantized, "fewer rows")
     alone = K.gated_backward(dh, gu, activation=act)
     assert alone.dgu is None and alone.amax is None
     _same_copies(alone.quantized, r.quantized, "alone")
@@ -479,7 +485,8 @@ def test_refusals_on_the_gpu():
            lambda: K.rmsnorm(x[:, :24].contiguous(), w[:24]), lambda: K.rmsnorm(x, w, want_y=False, quantize=False),
            lambda: K.rmsnorm(x, w, eps=-1.0), lambda: K.rmsnorm(_rand((1, 32800), 1), _rand((32800,), 1)),
            lambda: K.rmsnorm_backward(x, x, w, torch.ones(3, device="cuda")),
-           lambda: K.gated_backward(x, x), lambda: K.gated_backward(x, _rand((4, 128), 1), activation="tanh"),
+           lambda: K.gated_backward(x, x), lambda: K.gated_backward(x, _rand((3, 128), 1)),
+           lambda: K.gated_backward(x[:0], _rand((3, 128), 1)), lambda: K.gated_backward(x, _rand((4, 128), 1), activation="tanh"),
            lambda: K.gated_backward(x[:, :48], _rand((4, 96), 1)),
            lambda: gated_linear(x, _rand((65, 64), 1), qlinear_params=MXFP8),
            lambda: gated_linear(x.float(), _rand((64, 64), 1), qlinear_params=MXFP8),
@@ -629,4 +636,27 @@ def test_norm_gradient_of_many_rows_repeated(rows, cols):
     for _ in range(12):
         again = K.rmsnorm_backward(dy, h, gamma, rstd, dresidual=dres)
         assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    assert K.read_device_status() == 0
+
+
+def test_decoder_with_fused_blocks_stays_within_quantization_noise():
+    """The benchmark's decoder, small: the fused block against the same model in bf16, with the bounds that the plain
+    MXFP8 decoder is held to; and close to that decoder itself, from which only roundings separate it."""
+    import bench
+    dims = dict(layers=2, hidden=256, heads=4, kv_heads=2, ffn=512, vocab=512)
+    plain = config.get_qlinear_params_from_predefined(config.QuantizeRecipe.NON_QUANTIZE)
+    torch.manual_seed(0)
+    models = [bench.build_llama_decoder(torch, dims, p, fused_block=f) for p, f in ((MXFP8, True), (MXFP8, False), (plain, False), (plain, True))]
+    for m in models[1:]:
+        m.load_state_dict(models[0].state_dict())
+    ids, tgt = (torch.randint(0, 512, (2, 128), device="cuda") for _ in range(2))
+    losses, grads = [], []
+    for m in models:
+        loss = m(ids, tgt)
+        loss.backward()
+        losses.append(loss.item())
+        grads.append(torch.cat([p.grad.float().flatten() for _, p in sorted(m.named_parameters())]))
+    cos = [float(torch.nn.functional.cosine_similarity(g, grads[2], dim=0)) for g in grads]
+    assert all(abs(v - losses[2]) / losses[2] < 0.02 for v in losses), losses
+    assert min(cos) > 0.97, cos
     assert K.read_device_status() == 0

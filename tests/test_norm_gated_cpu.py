@@ -110,10 +110,12 @@ def test_gated_entry_points_refuse(p):
     rc = lib.mt_gemm_gated_nvfp4(p, p, None, p, p, None, p, 2, 128, 64, 0, out(h=p), None)
     _refused(rc, "abs-max")
 
-    def gb(dh=p, ds=64, gu=p, rows=2, F=64, act=0, dgu=p, q=None, s=None, ss=4, qt=None, st=None, sts=1):
-        return lib.mt_gated_backward(dh, ds, gu, rows, F, act, dgu, None, q, s, ss, None, qt, st, sts, None, None)
+    def gb(dh=p, ds=64, dr=2, gu=p, rows=2, F=64, act=0, dgu=p, q=None, s=None, ss=4, qt=None, st=None, sts=1):
+        return lib.mt_gated_backward(dh, ds, dr, gu, rows, F, act, dgu, None, q, s, ss, None, qt, st, sts, None, None)
 
     _refused(gb(dgu=None), "no output")
+    _refused(gb(dr=3), "rows for")
+    _refused(gb(dr=0), "rows for")
     _refused(gb(q=p), "codes need s")
     _refused(gb(q=p, s=p, ss=3), "codes need s")
     _refused(gb(q=p, s=p, qt=p), "need s_t")
@@ -212,6 +214,7 @@ class _ExactOp(Q.QuantizeOpBase):
     def gated_backward(self, dh, gu, qparams, activation):
         g, u = gu.float().chunk(2, -1)
         s = torch.sigmoid(g)
+        dh = torch.nn.functional.pad(dh, (0, 0, 0, gu.shape[0] - dh.shape[0]))     # rows without a gradient
         dgu = torch.cat([dh.float() * u * s * (1 + g * (1 - s)), dh.float() * g * s], -1)
         return self.quantize(dgu, qparams, return_transpose=True)
 
