@@ -525,13 +525,18 @@ def grouped_wgrad_mxfp8(qa_t, sa_t_swz, qb_t, sb_t_swz, m_splits, *, out_dtype=t
 def _on_tensor_device(fn):
     """Runs fn with the device of its first argument current, so that launches and allocations go
     there whatever device is current in the caller."""
+    name = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def wrapper(first, *args, **kw):
-        _require_cuda(first, "the first argument")
+    def wrapper(*args, **kw):
+        first = args[0] if args else kw.get(name)
+        if first is None:
+            raise _lib.MtError(f"{fn.__name__}: {name} is missing")
+        _require_cuda(first, name)
         if first.device.index == torch.cuda.current_device():
-            return fn(first, *args, **kw)
+            return fn(*args, **kw)
         with torch.cuda.device(first.device):
-            return fn(first, *args, **kw)
+            return fn(*args, **kw)
     return wrapper
 
 
@@ -698,10 +703,16 @@ def _gemm_gated(fmt, qa, sa_swz, amax_a, qb, sb_swz, amax_b, activation, sb_lin,
         raise _lib.MtError("gated projection: scale buffers are smaller than the GEMM layout of the operands")
     if not (want_h or want_gu or quantize_h):
         raise _lib.MtError("gated projection: no output requested")
+    if not (sa_swz.is_contiguous() and sb_swz.is_contiguous()):
+        raise _lib.MtError("gated projection: scale buffers must be contiguous")
+    if fmt == "nvfp4":
+        for name, t in (("amax_a", amax_a), ("amax_b", amax_b)):
+            if t is None or t.dtype != torch.float32 or t.numel() < 1:
+                raise _lib.MtError(f"gated projection: {name} must be an fp32 device scalar")
     sb_up = None
     if F % 128 and F:
         # the second projection's rows start inside a 128-row chunk of the stacked scales: a layout of their own
-        if sb_lin is None or sb_lin.shape[0] < 2 * F:
+        if sb_lin is None or sb_lin.dim() != 2 or sb_lin.shape[0] < 2 * F or sb_lin.shape[1] != K // block:
             raise _lib.MtError(f"gated projection: F = {F} is not a multiple of 128, which needs the row-major weight scales (sb_lin)")
         sb_up = swizzle_scales(sb_lin[F:2 * F])
     dev = qa.device

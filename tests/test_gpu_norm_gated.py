@@ -509,6 +509,21 @@ def test_refusals_on_the_gpu():
     assert K.read_device_status() == 0
 
 
+def test_operands_that_do_not_belong_together_are_refused():
+    q, _ = _operands(4, 96, 64, "mxfp8", 1)
+    with pytest.raises(_lib.MtError, match="sb_lin"):      # row-major scales of a shorter weight
+        K.gemm_gated_mxfp8(q[0].data, q[0].scale_swz, q[1].data, q[1].scale_swz, sb_lin=q[1].scale[:, :1])
+    with pytest.raises(_lib.MtError, match="contiguous"):
+        K.gemm_gated_mxfp8(q[0].data, torch.cat([q[0].scale_swz] * 2)[::2], q[1].data, q[1].scale_swz, sb_lin=q[1].scale)
+    f, _ = _operands(4, 128, 64, "nvfp4", 1)
+    for a, b in ((None, f[1].amax_row), (f[0].amax_row, None), (f[0].amax_row.double(), f[1].amax_row)):
+        with pytest.raises(_lib.MtError, match="fp32 device scalar"):
+            K.gemm_gated_nvfp4(f[0].data, f[0].scale_swz, a, f[1].data, f[1].scale_swz, b)
+    x, w = _rand((4, 64), 1), _rand((64,), 2)
+    a, b = K.rmsnorm(x, w), K.rmsnorm(x=x, weight=w)
+    assert torch.equal(a.y, b.y) and torch.equal(a.quantized.data, b.quantized.data)
+
+
 @pytest.mark.parametrize("rows,cols", [(700, 64), (1021, 2080), (640, 8192), (593, 4096), (600, 16384)])
 def test_norm_of_many_rows(rows, cols):
     """Rows enough for the persistent kernels, each CTA taking several: same bits as the same rows in small batches."""

@@ -177,6 +177,21 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
     assert current == [0]
 
 
+def test_first_argument_may_be_named(monkeypatch):
+    class FakeTensor:
+        is_cuda, device = True, torch.device("cuda", 0)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    t = FakeTensor()
+    f = kernels._on_tensor_device(lambda qa, other=1: (qa, other))
+    assert f(qa=t, other=2) == (t, 2) and f(t) == (t, 1)
+    with pytest.raises(_lib.MtError, match="qa is missing"):
+        f(other=2)
+    for g in (kernels.rmsnorm, kernels.rmsnorm_backward, kernels.gated_backward, kernels.gemm_gated_mxfp8, kernels.gemm_gated_nvfp4):
+        with pytest.raises(_lib.MtError, match="is missing"):
+            g()
+
+
 def test_activation_values_match_the_header():
     import re
     text = open(_lib.HEADER_PATHS[0]).read()
