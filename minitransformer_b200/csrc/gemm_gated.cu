@@ -54,6 +54,19 @@ __device__ __forceinline__ float gated_act_any(int act, float g) {
 // ------------------------------------------------------------------------------------------
 // M <= 128
 // ------------------------------------------------------------------------------------------
+// 32 lanes x 8 consecutive 32-bit columns of tensor memory.
+__device__ __forceinline__ void tc_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr) : "memory");
+}
+
+// An epilogue warp takes 32 features of 8 tokens at a time, four warps share the tokens of 32 features. It is a CTA's only
+// one, so nothing hides it: with one warp for all tokens, 32 at a time, one token on 14336 x 4096 (MXFP8) took 22.5 us
+// instead of 20.9, 128 tokens 30.6 instead of 26.5; with 16 at a time 21.6 and 26.8.
+constexpr int GR_TOKENS = 8, GR_SHARE = 4;
+constexpr int GR_THREADS = 64 + 128 * GR_SHARE;
+
 template <int kFormat, int BT, int STAGES>
 struct GatedRowsCfg {
   static constexpr int CH = (kFormat == FMT_NVFP4) ? 4 : 1;
@@ -75,9 +88,9 @@ struct GatedRowsCfg {
   static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory over-subscribed");
 };
 
-// One CTA per 128 features. 192 threads: TMA producer warp, MMA warp, four epilogue warps.
+// One CTA per 128 features: TMA producer warp, MMA warp, epilogue warps.
 template <int kFormat, int BT, int STAGES>
-__global__ void __launch_bounds__(G_THREADS, 1)
+__global__ void __launch_bounds__(GR_THREADS, 1)
     gemm_gated_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
                            const __grid_constant__ CUtensorMap map_u, const GatedArgs a) {
   using Cfg = GatedRowsCfg<kFormat, BT, STAGES>;
@@ -165,7 +178,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     __syncwarp();
   } else {
     // epilogue: lane <-> feature, warp <-> one 1x32 block of h per token
-    const int qd = warp & 3;
+    const int qd = warp & 3, part = (warp - 2) >> 2;
     const float alpha = gated_alpha(a);
     const int64_t f = f0 + qd * 32 + lane;
     const bool f_ok = f < a.F;
@@ -177,16 +190,16 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       uint8_t* chunk = a.s_swz + (int64_t)tile * 512;   // tokens of one 128-row block, blocks 4 tile ..
       const int M = (int)a.M;
 #pragma unroll 1
-      for (int c = 0; c < M; c += 32) {
-        uint32_t g[32], u[32];
-        tc_ld_32x32(lane_base + Cfg::TMEM_G + c, g);
-        tc_ld_32x32(lane_base + Cfg::TMEM_U + c, u);
+      for (int c = part * GR_TOKENS; c < M; c += GR_SHARE * GR_TOKENS) {
+        uint32_t g[GR_TOKENS], u[GR_TOKENS];
+        tc_ld_32x8(lane_base + Cfg::TMEM_G + c, g);
+        tc_ld_32x8(lane_base + Cfg::TMEM_U + c, u);
         tc_wait_ld();
-        const int n = min(32, M - c);     // (columns beyond the last token hold zeros: their rows of x are not there)
+        const int n = min(GR_TOKENS, M - c);     // (columns beyond the last token hold zeros: their rows of x are not there)
         if (a.gu != nullptr && f_ok) {
           __nv_bfloat16* p = a.gu + (int64_t)c * 2 * a.F + f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < GR_TOKENS; ++i) {
             if (i < n) {
               p[0] = __float2bfloat16_rn(alpha * __uint_as_float(g[i]));
               p[a.F] = __float2bfloat16_rn(alpha * __uint_as_float(u[i]));
@@ -194,23 +207,23 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             p += 2 * a.F;
           }
         }
-        // h of 32 tokens, all independent of one another; bf16 bits in the upper half of the word
+        // h of the tokens, all independent of one another; bf16 bits in the upper half of the word
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < GR_TOKENS; ++i) {
           const float h = gated_act_any(a.act, alpha * __uint_as_float(g[i])) * (alpha * __uint_as_float(u[i]));
           g[i] = f_ok ? static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(h))) << 16 : 0u;
         }
         if (a.h != nullptr && f_ok) {
           __nv_bfloat16* p = a.h + (int64_t)c * a.F + f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < GR_TOKENS; ++i) {
             if (i < n) *p = __ushort_as_bfloat16(static_cast<unsigned short>(g[i] >> 16));
             p += a.F;
           }
         }
         if (a.amax != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < GR_TOKENS; ++i)
             if (i < n) am.f = fmaxf(am.f, fabsf(__uint_as_float(g[i])));
         }
         if (a.q != nullptr) {
@@ -218,7 +231,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           // NaN is dropped as in mt_quantize_mxfp8) and computes its scale once
           uint32_t top = 0;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < GR_TOKENS; ++i) {
             const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(__uint_as_float(g[i])), 0.0f)));
             if (lane == i) top = m;
           }
@@ -226,13 +239,13 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           const uint32_t sb = mx_scale(top >> 16, enc);
           uint8_t* p = a.q + (int64_t)c * a.F + f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < GR_TOKENS; ++i) {
             const float e = __uint_as_float(__shfl_sync(0xffffffffu, enc, i) << 16);
             if (i < n && f_ok) *p = __nv_cvt_float_to_fp8(__uint_as_float(g[i]) * e, __NV_SATFINITE, __NV_E4M3);
             p += a.F;
           }
           const int t = c + lane;
-          if (t < M) {
+          if (lane < n) {
             const bool in = (int64_t)kb * 32 < a.F;
             if (in && a.s != nullptr) a.s[t * a.s_stride + kb] = static_cast<uint8_t>(sb);
             if (a.s_swz != nullptr) chunk[sf_chunk_offset(t, kb)] = in ? static_cast<uint8_t>(sb) : 0;
@@ -240,9 +253,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         }
       }
       if (a.s_swz != nullptr) {   // rows without a token, and the chunks up to the padded count
-        for (int t = (int)a.M + lane; t < 128; t += 32) chunk[sf_chunk_offset(t, kb)] = 0;
+        for (int t = (int)a.M + part * 32 + lane; t < 128; t += GR_SHARE * 32) chunk[sf_chunk_offset(t, kb)] = 0;
         if (tile == a.tiles_n - 1)
-          for (int64_t i = (a.tiles_n * 512) / 16 + qd * 32 + lane; i < a.kc_h * 32; i += 128)
+          for (int64_t i = (a.tiles_n * 512) / 16 + (warp - 2) * 32 + lane; i < a.kc_h * 32; i += 128 * GR_SHARE)
             *reinterpret_cast<uint4*>(a.s_swz + i * 16) = make_uint4(0, 0, 0, 0);
       }
       if (a.amax != nullptr) amax_publish(a.amax, am, lane);
@@ -527,7 +540,7 @@ static int launch_gated_rows(const CUtensorMap& mx, const CUtensorMap& mg, const
     MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC));
     attr_set[slot] = true;
   }
-  MT_CUDA(launch_pdl(kern, dim3(a.tiles_n), dim3(G_THREADS), (size_t)Cfg::SMEM_ALLOC, st, mx, mg, mu, a));
+  MT_CUDA(launch_pdl(kern, dim3(a.tiles_n), dim3(GR_THREADS), (size_t)Cfg::SMEM_ALLOC, st, mx, mg, mu, a));
   return MT_OK;
 }
 
@@ -572,11 +585,10 @@ static int launch_gated(const uint8_t* x, const uint8_t* wg, const uint8_t* wu, 
   if (rc != MT_OK) return rc;
   a.tiles_n = (int)((a.F + 127) / 128);
   if (small) {
-    // As many stages as shared memory holds: one token on 14336 x 4096 (MXFP8) takes 30.3 / 24.6 / 23.6 / 22.7 us with
-    // 2 / 3 / 4 / 5 (5.4 TB/s; what is left of 18.8 us at the copy rate is the launch, the first loads and the
-    // epilogue of a single wave). A 16-token variant with 6 stages was no faster.
+    // As many stages as shared memory holds: with 2 / 3 / 4 / 5 one token on 14336 x 4096 (MXFP8) took 30.3 / 24.6 / 23.6 /
+    // 22.7 us, 64 tokens with 4 / 5 24.2 / 23.4. A variant with 16 tokens on the column side and 6 stages was no faster.
     if (bt == 32) return launch_gated_rows<kFormat, 32, 5>(m[0], m[1], m[2], a, st);
-    if (bt == 64) return launch_gated_rows<kFormat, 64, 4>(m[0], m[1], m[2], a, st);
+    if (bt == 64) return launch_gated_rows<kFormat, 64, kFormat == FMT_NVFP4 ? 4 : 5>(m[0], m[1], m[2], a, st);
     if (bt == 96) return launch_gated_rows<kFormat, 96, 4>(m[0], m[1], m[2], a, st);
     return launch_gated_rows<kFormat, 128, 4>(m[0], m[1], m[2], a, st);
   }
