@@ -8,15 +8,17 @@
 //
 // Two kernels, by the number of rows M of x:
 //
-// gemm_gated_rows_kernel (M <= 128, decoding): the weights are read once and dominate, so they
-// take the 128-row side of the MMA and the tokens the column side (N = M rounded up to 32):
-// the tensor time shrinks with M and the pipeline holds almost only weight bytes. A CTA owns 128
-// features; its accumulators [128 features x tokens] put one feature in each lane, so a warp
-// owns one 1x32 block of h for every token.
+// gemm_gated_rows_kernel (decoding, short prompts): the weights dominate, so they take the 128-row side of the
+// MMA and the tokens the column side (32 to 128 of them): the tensor time shrinks with the tokens and the pipeline
+// holds almost only weight bytes. A CTA owns 128 features; its accumulators [128 features x tokens] put one
+// feature in each lane, so a warp owns one 1x32 block of h for every token. Bound by reading the weights: one
+// token on 14336 x 4096 takes 20.9 us (MXFP8; 121 MB, 18.8 us at the measured copy rate) or 13.1 us (NVFP4; 66 MB,
+// 10.2 us).
 //
-// gemm_gated_pair_kernel (M > 128): a CTA pair (cta_group::2) per 256 rows x 128 features. The B
-// tile of 256 rows is [128 rows of Wg; 128 rows of Wu], one half loaded by either CTA, so g and u
-// of a feature end up 128 accumulator columns apart in the same lane.
+// gemm_gated_pair_kernel (the rest): a CTA pair (cta_group::2) per 256 rows x 128 features. The B tile of
+// 256 rows is [128 rows of Wg; 128 rows of Wu], one half loaded by either CTA, so g and u of a feature end up 128
+// accumulator columns apart in the same lane. Bound by the tensor pipe (89 % busy in the NVFP4 form): 8192 x 4096 x 14336
+// takes 342 us (NVFP4, 5.6 PFLOP/s) or 645 us (MXFP8, 3.0) for h alone, 392 and 681 with [g | u] as well.
 //
 // Every wait on an mbarrier is bounded, as in the plain GEMM kernels.
 #include <algorithm>
@@ -47,12 +49,8 @@ __device__ __forceinline__ float gated_alpha(const GatedArgs& a) {
   return a.amax_a != nullptr ? __fdiv_rn(__fmul_rn(*a.amax_a, *a.amax_b), 6.0f * 6.0f * 448.0f * 448.0f) : 1.0f;
 }
 
-__device__ __forceinline__ float gated_act_any(int act, float g) {
-  return act == MT_ACT_SILU ? gated_act<MT_ACT_SILU>(g) : gated_act<MT_ACT_GELU>(g);
-}
-
 // ------------------------------------------------------------------------------------------
-// M <= 128
+// few tokens
 // ------------------------------------------------------------------------------------------
 // 32 lanes x 8 consecutive 32-bit columns of tensor memory.
 __device__ __forceinline__ void tc_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -88,7 +86,7 @@ struct GatedRowsCfg {
   static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory over-subscribed");
 };
 
-// One CTA per 128 features: TMA producer warp, MMA warp, epilogue warps.
+// One CTA per 128 features and BT tokens (blockIdx.y): TMA producer warp, MMA warp, epilogue warps.
 template <int kFormat, int BT, int STAGES>
 __global__ void __launch_bounds__(GR_THREADS, 1)
     gemm_gated_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
@@ -104,7 +102,7 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NUM_BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x;
+  const int tile = blockIdx.x, m0 = (int)blockIdx.y * BT;
   const int64_t f0 = (int64_t)tile * 128;
   const int num_k = (int)((a.K_bytes + G_BLOCK_KB - 1) / G_BLOCK_KB);
 
@@ -137,12 +135,12 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
         mbar_expect_tx(&full_bar[s], Cfg::STAGE_BYTES);
         tma_load_2d(smem + Cfg::OFF_G + s * Cfg::W_BYTES, &map_g, &full_bar[s], k * G_BLOCK_KB, (int32_t)f0);
         tma_load_2d(smem + Cfg::OFF_U + s * Cfg::W_BYTES, &map_u, &full_bar[s], k * G_BLOCK_KB, (int32_t)f0);
-        tma_load_2d(smem + Cfg::OFF_T + s * Cfg::T_BYTES, &map_x, &full_bar[s], k * G_BLOCK_KB, 0);
+        tma_load_2d(smem + Cfg::OFF_T + s * Cfg::T_BYTES, &map_x, &full_bar[s], k * G_BLOCK_KB, m0);
         uint8_t* sf = smem + Cfg::OFF_SF + s * 3 * Cfg::SF_BYTES;
         const int64_t chunk = (int64_t)tile * a.kc + (int64_t)k * CH;
         bulk_load_1d(sf, a.sb_gate + chunk * 512, Cfg::SF_BYTES, &full_bar[s]);
         bulk_load_1d(sf + Cfg::SF_BYTES, a.sb_up + chunk * 512, Cfg::SF_BYTES, &full_bar[s]);
-        bulk_load_1d(sf + 2 * Cfg::SF_BYTES, a.sa + (int64_t)k * CH * 512, Cfg::SF_BYTES, &full_bar[s]);
+        bulk_load_1d(sf + 2 * Cfg::SF_BYTES, a.sa + ((m0 >> 7) * a.kc + (int64_t)k * CH) * 512, Cfg::SF_BYTES, &full_bar[s]);
         if (++s == STAGES) { s = 0; ph ^= 1; }
       }
     }
@@ -166,9 +164,10 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
         for (int j = 0; j < 4; ++j) {
           const uint32_t idesc = make_idesc(kFormat, BT, j);
           const uint32_t sf = tmem_base + Cfg::TMEM_SF + (kFormat == FMT_NVFP4 ? 4 * j : 0);
+          const uint32_t sft = sf + 8 * CH + ((m0 >> 5) & 3);   // 32 rows of a chunk per column
           const uint32_t acc = (k > 0 || j > 0) ? 1u : 0u;
-          issue_mma<kFormat>(tmem_base + Cfg::TMEM_G, gdesc + 2 * j, tdesc + 2 * j, idesc, sf, sf + 8 * CH, acc);
-          issue_mma<kFormat>(tmem_base + Cfg::TMEM_U, udesc + 2 * j, tdesc + 2 * j, idesc, sf + 4 * CH, sf + 8 * CH, acc);
+          issue_mma<kFormat>(tmem_base + Cfg::TMEM_G, gdesc + 2 * j, tdesc + 2 * j, idesc, sf, sft, acc);
+          issue_mma<kFormat>(tmem_base + Cfg::TMEM_U, udesc + 2 * j, tdesc + 2 * j, idesc, sf + 4 * CH, sft, acc);
         }
         tc_commit(&empty_bar[s]);
         if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -180,6 +179,7 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
     // epilogue: lane <-> feature, warp <-> one 1x32 block of h per token
     const int qd = warp & 3, part = (warp - 2) >> 2;
     const float alpha = gated_alpha(a);
+    const bool silu = a.act == MT_ACT_SILU;
     const int64_t f = f0 + qd * 32 + lane;
     const bool f_ok = f < a.F;
     const int kb = (int)(f0 >> 5) + qd;
@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
     if (mbar_wait_bounded(acc_full, 0, abort_flag, a.status, DS_ACC_FULL_WAIT)) {
       tc_fence_after();
       const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(qd * 32) << 16);
-      uint8_t* chunk = a.s_swz + (int64_t)tile * 512;   // tokens of one 128-row block, blocks 4 tile ..
-      const int M = (int)a.M;
+      uint8_t* chunk = a.s_swz + ((m0 >> 7) * a.kc_h + tile) * 512;   // tokens of one 128-row block, blocks 4 tile ..
+      const int M = (int)min((int64_t)BT, a.M - m0);                  // of this CTA
 #pragma unroll 1
       for (int c = part * GR_TOKENS; c < M; c += GR_SHARE * GR_TOKENS) {
         uint32_t g[GR_TOKENS], u[GR_TOKENS];
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
         tc_wait_ld();
         const int n = min(GR_TOKENS, M - c);     // (columns beyond the last token hold zeros: their rows of x are not there)
         if (a.gu != nullptr && f_ok) {
-          __nv_bfloat16* p = a.gu + (int64_t)c * 2 * a.F + f;
+          __nv_bfloat16* p = a.gu + (int64_t)(m0 + c) * 2 * a.F + f;
 #pragma unroll
           for (int i = 0; i < GR_TOKENS; ++i) {
             if (i < n) {
@@ -210,11 +210,12 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
         // h of the tokens, all independent of one another; bf16 bits in the upper half of the word
 #pragma unroll
         for (int i = 0; i < GR_TOKENS; ++i) {
-          const float h = gated_act_any(a.act, alpha * __uint_as_float(g[i])) * (alpha * __uint_as_float(u[i]));
+          const float v = alpha * __uint_as_float(g[i]);
+          const float h = (silu ? gated_act<MT_ACT_SILU>(v) : gated_act<MT_ACT_GELU>(v)) * (alpha * __uint_as_float(u[i]));
           g[i] = f_ok ? static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(h))) << 16 : 0u;
         }
         if (a.h != nullptr && f_ok) {
-          __nv_bfloat16* p = a.h + (int64_t)c * a.F + f;
+          __nv_bfloat16* p = a.h + (int64_t)(m0 + c) * a.F + f;
 #pragma unroll
           for (int i = 0; i < GR_TOKENS; ++i) {
             if (i < n) *p = __ushort_as_bfloat16(static_cast<unsigned short>(g[i] >> 16));
@@ -237,14 +238,14 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
           }
           uint32_t enc;
           const uint32_t sb = mx_scale(top >> 16, enc);
-          uint8_t* p = a.q + (int64_t)c * a.F + f;
+          uint8_t* p = a.q + (int64_t)(m0 + c) * a.F + f;
 #pragma unroll
           for (int i = 0; i < GR_TOKENS; ++i) {
             const float e = __uint_as_float(__shfl_sync(0xffffffffu, enc, i) << 16);
             if (i < n && f_ok) *p = __nv_cvt_float_to_fp8(__uint_as_float(g[i]) * e, __NV_SATFINITE, __NV_E4M3);
             p += a.F;
           }
-          const int t = c + lane;
+          const int t = m0 + c + lane;
           if (lane < n) {
             const bool in = (int64_t)kb * 32 < a.F;
             if (in && a.s != nullptr) a.s[t * a.s_stride + kb] = static_cast<uint8_t>(sb);
@@ -253,10 +254,11 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
         }
       }
       if (a.s_swz != nullptr) {   // rows without a token, and the chunks up to the padded count
-        for (int t = (int)a.M + part * 32 + lane; t < 128; t += GR_SHARE * 32) chunk[sf_chunk_offset(t, kb)] = 0;
-        if (tile == a.tiles_n - 1)
-          for (int64_t i = (a.tiles_n * 512) / 16 + (warp - 2) * 32 + lane; i < a.kc_h * 32; i += 128 * GR_SHARE)
-            *reinterpret_cast<uint4*>(a.s_swz + i * 16) = make_uint4(0, 0, 0, 0);
+        if (blockIdx.y == gridDim.y - 1)
+          for (int t = m0 + M + part * 32 + lane; t < ((m0 >> 7) + 1) * 128; t += GR_SHARE * 32) chunk[sf_chunk_offset(t, kb)] = 0;
+        if (tile == a.tiles_n - 1 && (m0 & 127) == 0)
+          for (int64_t i = 32 + (warp - 2) * 32 + lane; i < (a.kc_h - tile) * 32; i += 128 * GR_SHARE)
+            *reinterpret_cast<uint4*>(chunk + i * 16) = make_uint4(0, 0, 0, 0);
       }
       if (a.amax != nullptr) amax_publish(a.amax, am, lane);
     }
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(GR_THREADS, 1)
 }
 
 // ------------------------------------------------------------------------------------------
-// M > 128
+// many tokens
 // ------------------------------------------------------------------------------------------
 // 16 row blocks (4096 rows) per band: at 8192 x 4096 x 14336 with both bf16 outputs, bands of 1 / 4 / 8 / 16 / 32 took
 // 474 / 442 / 422 / 412 / 411 us (NVFP4) and 870 / 741 / 715 / 702 / 704 us (MXFP8, whose weight alone fills L2).
@@ -540,7 +542,7 @@ static int launch_gated_rows(const CUtensorMap& mx, const CUtensorMap& mg, const
     MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC));
     attr_set[slot] = true;
   }
-  MT_CUDA(launch_pdl(kern, dim3(a.tiles_n), dim3(GR_THREADS), (size_t)Cfg::SMEM_ALLOC, st, mx, mg, mu, a));
+  MT_CUDA(launch_pdl(kern, dim3(a.tiles_n, (unsigned)((a.M + BT - 1) / BT)), dim3(GR_THREADS), (size_t)Cfg::SMEM_ALLOC, st, mx, mg, mu, a));
   return MT_OK;
 }
 
@@ -577,13 +579,16 @@ static int launch_gated(const uint8_t* x, const uint8_t* wg, const uint8_t* wu, 
   CUtensorMap m[6];
   const uint64_t ld = (uint64_t)a.K_bytes;
   constexpr uint32_t CH = kFormat == FMT_NVFP4 ? 4 : 1;
-  const bool small = a.M <= 128;
-  const uint32_t bt = small ? (uint32_t)((a.M + 31) / 32 * 32) : 128u;
+  a.tiles_n = (int)((a.F + 127) / 128);
+  // Blocks of 64 tokens where one wave holds them all: the fewer tokens a CTA has, the sooner it is done. 1000 tokens on
+  // 768 x 2048: 7.9 us in 64-token blocks, 9.4 us in 256-row pairs; 128 on 4096 x 1024: 5.7 us in two blocks, 7.5 us in one.
+  const bool spread = a.M > 64 && (a.M + 63) / 64 * a.tiles_n <= mx_sm_count();
+  const bool small = spread || a.M <= 128;
+  const uint32_t bt = spread ? 64u : small ? (uint32_t)((a.M + 31) / 32 * 32) : 128u;
   int rc = make_tensor_map_2d(&m[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, ld, (uint64_t)a.M, ld, G_BLOCK_KB, bt, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == MT_OK) rc = make_tensor_map_2d(&m[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wg, ld, (uint64_t)a.F, ld, G_BLOCK_KB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == MT_OK) rc = make_tensor_map_2d(&m[2], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wu, ld, (uint64_t)a.F, ld, G_BLOCK_KB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != MT_OK) return rc;
-  a.tiles_n = (int)((a.F + 127) / 128);
   if (small) {
     // As many stages as shared memory holds: with 2 / 3 / 4 / 5 one token on 14336 x 4096 (MXFP8) took 30.3 / 24.6 / 23.6 /
     // 22.7 us, 64 tokens with 4 / 5 24.2 / 23.4. A variant with 16 tokens on the column side and 6 stages was no faster.

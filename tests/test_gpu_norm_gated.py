@@ -230,6 +230,14 @@ def test_gated_projection_matches_formula(M, F, Kd, fmt, act):
     assert K.read_device_status() == 0
 
 
+@pytest.mark.parametrize("M,F,Kd", [(127, 160, 96), (191, 224, 64), (193, 1376, 96), (449, 32, 32), (640, 1792, 544), (2000, 416, 160),
+                                    (90, 9600, 64), (100, 10016, 96), (193, 8192, 64), (700, 2080, 128), (1601, 800, 96)])
+@pytest.mark.parametrize("fmt", ["mxfp8", "nvfp4"])
+def test_gated_projection_on_both_sides_of_one_wave(M, F, Kd, fmt):
+    """64-token blocks as long as one wave holds them, whole columns of tokens or 256-row pairs beyond."""
+    test_gated_projection_matches_formula(M, F, Kd, fmt, "silu")
+
+
 def test_gated_projection_equals_the_plain_gemm():
     """The projections are those of the library's GEMM, rounded once."""
     for M in (40, 300):
