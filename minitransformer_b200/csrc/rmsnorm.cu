@@ -6,9 +6,10 @@
 //   y = bf16(h * rstd * gamma)          products in fp32, rounded once
 //   copy: E4M3 codes and E8M0 scales of y in 1x32 blocks, bit for bit what mt_quantize_mxfp8 makes of y
 //
-// Both directions move every element once and do a few operations on it: they are bound by HBM
-// (forward with residual and codes: 2 + 2 read, 2 + 1 written per element; backward 2 + 2 (+ 2)
-// read, 2 written).
+// Both directions move every element once and do a few operations on it: they are bound by HBM. 8192 x 4096 with a
+// residual: h and y 48 us (268 MB, 5.6 TB/s), with row-wise codes 57 us (303 MB, 5.3 TB/s), with both copies 66 us
+// (340 MB, 5.2 TB/s); 8192 x 8192 with both copies 147 us. Gradient of 8192 x 8192 with a residual: 84 us (537 MB,
+// 6.4 TB/s). A plain copy reaches 6.46 TB/s. One token of 4096 columns: 2.4 us, a launch.
 #include "tile_quant.cuh"
 
 namespace mt {
@@ -213,7 +214,8 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_rows_kernel(const RmsNorm
 // ways in registers. The clusters are persistent: a warp asks for its tiles of the next panel (TMA, one mbarrier
 // per warp) as soon as it holds the present ones, so that they arrive while it waits for its cluster,
 // quantizes and stores. The sums travel by st.async onto an mbarrier of the receiving CTA: a cluster barrier's
-// release would wait for the stores of h, y and the copies as well. Two sets of sums and barriers alternate: a
+// release would wait for the stores of h, y and the copies as well (81 us instead of 69 on 8192 x 4096). h is stored
+// before the exchange, y and the copies after it. Three CTAs per SM at 80 registers: 77 us instead of 66. Two sets of sums and barriers alternate: a
 // CTA that has received all sums of panel n + 1 knows that everybody has read those of panel n.
 // Panels beyond the last row (up to 128 rows) and the last panel write the scales' padding.
 constexpr int RN_PANEL_MAX_COLS = 8192;
@@ -595,7 +597,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_grad_kernel(const RmsNormGradArg
   }
 }
 
-// The same with the rows on their way ahead of time: a ring of shared-memory stages, each one row of dy, h and dres
+// The same with the rows on their way ahead of time (138 -> 84 us on 8192 x 8192 with a residual): a ring of shared-memory stages, each one row of dy, h and dres
 // fetched by bulk copies (one mbarrier per stage). A row needs one barrier (inside the sum); once a thread
 // has passed the one of row n + 1, everybody is done with row n, and its stage is filled again.
 template <int V, int kMaxThreads, int kMinCtas>
@@ -723,8 +725,9 @@ __global__ void __launch_bounds__(32 * RN_SUM_GROUPS) rmsnorm_dgamma_kernel(cons
 // Threads per row for V vectors per thread (a multiple of 64: whole groups of four segments).
 static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / V + 63) / 64 * 64); }
 
-// CTAs per SM that share its memory for their rings, one vector of 8 columns per thread. Two CTAs of 512 threads on 4096 columns and one of 1024 on 8192: with two vectors per thread (two CTAs of
-// 512) the gradient of 8192 x 8192 took 119 us instead of 85.
+// CTAs per SM that share its memory for their rings, one vector of 8 columns per thread: two CTAs of 512 threads on
+// 4096 columns, one of 1024 on 8192. With two vectors per thread (two CTAs of 512) the gradient of 8192 x 8192 took
+// 119 us instead of 84.
 static int rn_ring_ctas_per_sm(int64_t cols) { return cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1; }
 static int rn_ring_stages(int64_t cols, int64_t stage) {
   const int64_t n = RN_RING_BYTES / rn_ring_ctas_per_sm(cols) / stage;

@@ -4,9 +4,10 @@
 //
 // Lane l holds rows 8 (l / 8) .. +7 of columns 8 (l % 8) .. +7 as packed bf16x2, w[row][column pair].
 // A 1x32 block along a row is four lanes (l xor 1, 2), a block along a column four lanes (l xor 8,
-// 16): two shuffles per row and per column pair. Loads and row-wise stores are 16 and 8 bytes per
-// lane in 128- and 64-byte runs, transposed stores 8 bytes per lane in runs of whole 32-byte
-// sectors. Codes, scales and padding are bit for bit those of mt_quantize_mxfp8.
+// 16). Row-wise stores are 8 bytes per lane in 64-byte runs, transposed stores 8 bytes per lane in
+// runs of whole 32-byte sectors; where the row count is not a multiple of 8 these runs start anywhere and leave as aligned
+// words (gated gradient, 3511 / 3512 x 4800: 76 / 50 us). Codes, scales and padding are bit for bit those of
+// mt_quantize_mxfp8.
 #pragma once
 
 #include "quantize_common.cuh"
