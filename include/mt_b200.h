@@ -364,7 +364,7 @@ int mt_peer_reduce_bf16(const void* stage, int n, int64_t rows, int64_t cols, vo
  *   q, s (stride s_stride), s_swz, q_t, s_t (stride s_t_stride), s_t_swz: MXFP8 copies of y as
  *   mt_quantize_mxfp8 makes them (cols % 32 == 0; with q_t at most 8192 columns, beyond that
  *   MT_ERR_UNSUPPORTED).
- * h may be the same buffer as x or residual. */
+ * h may be the buffer of x or of residual, if that one has a row stride of cols. */
 int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
                        const void* gamma, int gamma_dtype, int64_t rows, int64_t cols, float eps,
                        void* h, float* rstd, void* y, float* amax,
@@ -375,7 +375,7 @@ int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* residual, in
  *   dx = rstd * (dy * gamma - xhat * mean(dy * gamma * xhat)) + dres, dgamma = sum over rows of dy * xhat,
  *   xhat = h * rstd.
  * dres (optional): gradient that reaches h from elsewhere. dx bf16 [rows, cols] contiguous, may be dres's
- * buffer; dgamma fp32 [cols], overwritten, the same bits for the same inputs on the same device.
+ * buffer if that has a row stride of cols; dgamma fp32 [cols], overwritten, the same bits for the same inputs on the same device.
  * workspace: mt_rmsnorm_backward_workspace(rows, cols) bytes (for the current device). */
 int64_t mt_rmsnorm_backward_workspace(int64_t rows, int64_t cols);
 int mt_rmsnorm_backward(const void* dy, int64_t dy_stride, const void* h, int64_t h_stride,

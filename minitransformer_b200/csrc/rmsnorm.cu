@@ -774,6 +774,8 @@ extern "C" int mt_rmsnorm_forward(const void* x, int64_t x_stride, const void* r
   MT_REQUIRE(!residual || (r_stride >= cols && row_aligned(residual, r_stride)), "%s: residual needs 16-byte aligned rows", name);
   MT_REQUIRE(!residual || h, "%s: a residual needs an output for the sum", name);
   MT_REQUIRE(residual || !h, "%s: without a residual there is no sum to write", name);
+  MT_REQUIRE(!h || ((h != x || x_stride == cols) && (h != residual || r_stride == cols)),
+             "%s: h in the place of an input needs that input's row stride to be cols", name);
   MT_REQUIRE(aligned16(gamma) && aligned16(h) && aligned16(y), "%s: pointers must be 16-byte aligned", name);
   int rc = mx_outputs_ok(name, rows, cols, q, s, s_stride, s_swz, q_t, s_t, s_t_stride, s_t_swz);
   if (rc != MT_OK) return rc;
@@ -825,6 +827,7 @@ extern "C" int mt_rmsnorm_backward(const void* dy, int64_t dy_stride, const void
   MT_REQUIRE(dy_stride >= cols && row_aligned(dy, dy_stride) && h_stride >= cols && row_aligned(h, h_stride),
              "%s: dy and h need 16-byte aligned rows", name);
   MT_REQUIRE(!dres || (dres_stride >= cols && row_aligned(dres, dres_stride)), "%s: dres needs 16-byte aligned rows", name);
+  MT_REQUIRE(dx != dres || dres_stride == cols, "%s: dx in the place of dres needs a row stride of cols", name);
   MT_REQUIRE(aligned16(gamma) && aligned16(dx), "%s: pointers must be 16-byte aligned", name);
   MT_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= mt_rmsnorm_backward_workspace(rows, cols),
              "%s: workspace of %lld bytes is too small (mt_rmsnorm_backward_workspace)", name, (long long)workspace_bytes);

@@ -517,6 +517,32 @@ def test_refusals_on_the_gpu():
     assert K.read_device_status() == 0
 
 
+@pytest.mark.parametrize("rows,cols", [(5, 96), (700, 2080), (300, 4096)])
+@pytest.mark.parametrize("transpose", [True, False])
+@pytest.mark.parametrize("into", ["x", "residual"])
+def test_norm_in_place(rows, cols, transpose, into):
+    """The sum in the place of x or of the residual, the gradient in the place of dres (C ABI)."""
+    x, r, w, dy, d = _rand((rows, cols), 1), _rand((rows, cols), 2), _rand((cols,), 3), _rand((rows, cols), 4), _rand((rows, cols), 5)
+    want = K.rmsnorm(x, w, residual=r, return_transpose=transpose)
+    c = K._mxfp8_outputs(rows, cols, transpose, x.device)
+    y, rstd, stream = torch.empty_like(x), torch.empty(rows, device="cuda"), torch.cuda.current_stream().cuda_stream
+    h = {"x": x, "residual": r}[into]
+    ptr = K._ptr
+    _lib.call("mt_rmsnorm_forward", ptr(x), cols, ptr(r), cols, ptr(w), _lib.MT_BF16, rows, cols, 1e-5, ptr(h), ptr(rstd), ptr(y),
+              None, ptr(c.data), ptr(c.scale), cols // 32, ptr(c.scale_swz), ptr(c.data_t), ptr(c.scale_t), (rows + 31) // 32,
+              ptr(c.scale_t_swz), stream)
+    assert torch.equal(h, want.h) and torch.equal(y, want.y) and torch.equal(rstd, want.rstd)
+    _same_copies(c, want.quantized, "in place")
+    dx, dw = K.rmsnorm_backward(dy, h, w, rstd, dresidual=d)
+    dw2 = torch.empty_like(dw)
+    n = _lib.load().mt_rmsnorm_backward_workspace(rows, cols)
+    work = torch.empty(n, dtype=torch.uint8, device="cuda")
+    _lib.call("mt_rmsnorm_backward", ptr(dy), cols, ptr(h), cols, ptr(w), _lib.MT_BF16, ptr(rstd), ptr(d), cols, rows, cols, ptr(d),
+              ptr(dw2), ptr(work), n, stream)
+    assert torch.equal(d, dx) and torch.equal(dw2, dw)
+    assert K.read_device_status() == 0
+
+
 def test_operands_that_do_not_belong_together_are_refused():
     q, _ = _operands(4, 96, 64, "mxfp8", 1)
     with pytest.raises(_lib.MtError, match="sb_lin"):      # row-major scales of a shorter weight

@@ -66,6 +66,9 @@ def test_norm_entry_points_refuse(p):
     def bwd(dy=p, dys=64, h=p, hs=64, g=p, gd=0, rstd=p, dres=None, drs=0, rows=2, cols=64, dx=p, dg=p, ws=p, wb=1 << 20):
         return lib.mt_rmsnorm_backward(dy, dys, h, hs, g, gd, rstd, dres, drs, rows, cols, dx, dg, ws, wb, None)
 
+    _refused(fwd(r=p, rs=72, h=p), "row stride to be cols")
+    _refused(fwd(x=p, xs=128, r=p + 64, rs=64, h=p), "row stride to be cols")
+    _refused(bwd(dres=p, drs=72), "row stride of cols")
     _refused(bwd(cols=20), "multiple of 8")
     _refused(bwd(gd=3), "dtype")
     _refused(bwd(dg=None), "dgamma")
