@@ -1,9 +1,9 @@
 // Gradient of the gated activation: from dh and the saved projections [g | u],
 //   du = bf16(dh * act(g)),   dg = bf16(dh * u * act'(g))
 // and, from the same registers, the MXFP8 copies of [dg | du] that the dgrad and wgrad GEMMs read (row-wise and
-// transposed). 6 bytes read and 4 written per (row, feature): bound by HBM. 8192 x 14336 with both copies takes 241 us
-// (1204 MB, 5.0 TB/s), the bf16 gradient alone, which needs no quantization, 226 us (5.2 TB/s): three reads to
-// two writes come no nearer to the 6.46 TB/s of a plain copy. 1021 x 1376: 12.4 us (1024 x 1376: 7.7 us).
+// transposed). 6 bytes read and 4 written per (row, feature): bound by HBM. 8192 x 14336 with both copies takes 237 us (silu)
+// or 229 us (gelu) (1204 MB, 5.1 - 5.3 TB/s), the bf16 gradient alone 204 us (1174 MB, 5.8 TB/s; the same without the
+// arithmetic: 203 us, without the stores 101 us). 1021 x 1376: 12.4 us (1024 x 1376: 7.5 us).
 #include "gated_act.cuh"
 #include "tile_quant.cuh"
 
@@ -24,10 +24,15 @@ struct GatedGradArgs {
 // mbarrier per warp) and asks for the next ones as soon as it has computed dg and du into registers: they arrive
 // while the warp quantizes and stores. Scale bytes are collected in shared memory and leave as words. Measured and
 // left out: an L2 hint that lets the inputs go first (301 us instead of 241 on 8192 x 14336), warps that store by
-// themselves (218 instead of 117 on 4096 x 14336), dg and du in CTAs of their own for few tiles (1024 x 1376: 8.8 us).
+// themselves (slower, their scales leave as bytes), dg and du in CTAs of their own for few tiles (1024 x 1376: 8.8 us), scale chunks
+// written as whole lines (no change).
 constexpr int GG_SMEM = 8 * 3 * MX_TILE_BYTES + 128;
 
-template <int kAct, bool kRagged>
+// kDgu: the bf16 gradient or its abs-max is asked for; kCopies: the MXFP8 copies are. Spills cost more here than their
+// number says, since they queue behind the stores: one kernel for all of it, without the two __syncwarp that keep the
+// loads of a tile from being moved ahead all at once, spilled 22 registers and took 116 us instead of 110 on 4096 x
+// 14336 (copies), 226 instead of 204 on 8192 x 14336 (dgu alone).
+template <int kAct, bool kRagged, bool kDgu, bool kCopies>
 __global__ void __launch_bounds__(256, 2)
     gated_grad_kernel(const __grid_constant__ CUtensorMap map_dh, const __grid_constant__ CUtensorMap map_gu, const GatedGradArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -79,10 +84,11 @@ __global__ void __launch_bounds__(256, 2)
       wu[i][j] = f32x2_to_bf16x2(mul2(d2, act));
       wg[i][j] = f32x2_to_bf16x2(mul2(mul2(d2, bf16x2_to_f32x2(u[j])), grad));
     }
+    if (i % 4 == 3) __syncwarp();
   }
   mx_release_tile(&empty[warp], ph, &abort_flag, a.status);
   if (lane == 0 && tile + (int)gridDim.x < a.tiles) fetch(tile + gridDim.x);
-  if (a.dgu != nullptr) {
+  if (kDgu && a.dgu != nullptr) {
     const int64_t row = row0 + (lane >> 3) * 8, f = c0 + (lane & 7) * 8;
     const int nrow = f < a.F ? mx_valid_rows(a.rows, row) : 0;
     __nv_bfloat16* pg = a.dgu + row * 2 * a.F + f;
@@ -95,7 +101,7 @@ __global__ void __launch_bounds__(256, 2)
       pg += 2 * a.F;
     }
   }
-  if (a.amax != nullptr) {
+  if (kDgu && a.amax != nullptr) {
     const bool in = c0 + (lane & 7) * 8 < a.F;   // a tile across the border holds the first columns of u as g
     uint32_t am = 0;
 #pragma unroll
@@ -105,7 +111,7 @@ __global__ void __launch_bounds__(256, 2)
     const uint32_t bits = __reduce_max_sync(0xffffffffu, in ? __float_as_uint(absmax2_to_float(am)) : 0u);
     if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
   }
-  if (o.q == nullptr) continue;
+  if (!kCopies) continue;
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const MxTileScales sc = p ? mx_tile_store<kRagged>(o, wu, row0, a.F + c0, 2 * a.F)
@@ -156,17 +162,26 @@ __global__ void __launch_bounds__(256, 2)
   pdl_trigger();
 }
 
-template <int kAct, bool kRagged>
+template <int kAct, bool kRagged, bool kDgu, bool kCopies>
 static int launch_gated_grad(const CUtensorMap& mdh, const CUtensorMap& mgu, const GatedGradArgs& a, cudaStream_t st) {
+  auto kern = gated_grad_kernel<kAct, kRagged, kDgu, kCopies>;
   static bool attr_set[MT_MAX_DEVICES] = {};
   const int slot = current_device_slot();
   if (!attr_set[slot]) {
-    MT_CUDA(cudaFuncSetAttribute(gated_grad_kernel<kAct, kRagged>, cudaFuncAttributeMaxDynamicSharedMemorySize, GG_SMEM));
+    MT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GG_SMEM));
     attr_set[slot] = true;
   }
   const int grid = a.tiles < 2 * mx_sm_count() ? a.tiles : 2 * mx_sm_count();
-  MT_CUDA(launch_pdl(gated_grad_kernel<kAct, kRagged>, dim3(grid), dim3(256), (size_t)GG_SMEM, st, mdh, mgu, a));
+  MT_CUDA(launch_pdl(kern, dim3(grid), dim3(256), (size_t)GG_SMEM, st, mdh, mgu, a));
   return MT_OK;
+}
+template <int kAct>
+static int gated_grad(const CUtensorMap& mdh, const CUtensorMap& mgu, const GatedGradArgs& a, cudaStream_t st) {
+  const bool dgu = a.dgu != nullptr || a.amax != nullptr;
+  if (a.out.q == nullptr) return launch_gated_grad<kAct, false, true, false>(mdh, mgu, a, st);
+  if (a.rows % 8 != 0)
+    return dgu ? launch_gated_grad<kAct, true, true, true>(mdh, mgu, a, st) : launch_gated_grad<kAct, true, false, true>(mdh, mgu, a, st);
+  return dgu ? launch_gated_grad<kAct, false, true, true>(mdh, mgu, a, st) : launch_gated_grad<kAct, false, false, true>(mdh, mgu, a, st);
 }
 
 }  // namespace mt
@@ -203,8 +218,5 @@ extern "C" int mt_gated_backward(const void* dh, int64_t dh_stride, int64_t dh_r
   if (rc == MT_OK) rc = mx_tile_map(&mgu, gu, rows, 2 * F, 2 * F);
   if (rc != MT_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool ragged = rows % 8 != 0;
-  if (activation == MT_ACT_SILU)
-    return ragged ? launch_gated_grad<MT_ACT_SILU, true>(mdh, mgu, a, st) : launch_gated_grad<MT_ACT_SILU, false>(mdh, mgu, a, st);
-  return ragged ? launch_gated_grad<MT_ACT_GELU, true>(mdh, mgu, a, st) : launch_gated_grad<MT_ACT_GELU, false>(mdh, mgu, a, st);
+  return activation == MT_ACT_SILU ? gated_grad<MT_ACT_SILU>(mdh, mgu, a, st) : gated_grad<MT_ACT_GELU>(mdh, mgu, a, st);
 }
