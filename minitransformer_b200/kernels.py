@@ -643,6 +643,12 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residua
     return RmsNormResult(h, rstd, y if want_y else None, c if quantize else None, amax)
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(rows: int, cols: int, device_index: int) -> int:
+    """mt_rmsnorm_backward_workspace of the current device (its number of SMs counts), which is device_index."""
+    return int(_lib.load().mt_rmsnorm_backward_workspace(rows, cols))
+
+
 @_on_tensor_device
 def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, *,
                      dresidual: Optional[torch.Tensor] = None):
@@ -660,7 +666,7 @@ def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rs
     dev = dy.device
     dx = _empty2(M, C, torch.bfloat16, dev)
     dweight = _empty1(C, torch.float32, dev)
-    n = int(_lib.load().mt_rmsnorm_backward_workspace(M, C))
+    n = _norm_workspace(M, C, dev.index)
     work = _empty1(n, torch.uint8, dev) if n else None
     _lib.call("mt_rmsnorm_backward", dy.data_ptr(), _row_stride(dy), h.data_ptr(), _row_stride(h), weight.data_ptr(),
               _out_dtype_code(weight.dtype), rstd.data_ptr(), _ptr(dresidual),
@@ -716,20 +722,11 @@ def _gemm_gated(fmt, qa, sa_swz, amax_a, qb, sb_swz, amax_b, activation, sb_lin,
             raise _lib.MtError(f"gated projection: F = {F} is not a multiple of 128, which needs the row-major weight scales (sb_lin)")
         sb_up = swizzle_scales(sb_lin[F:2 * F])
     dev = qa.device
-    r = GatedResult()
-    o = _lib.GatedOutputs()
-    if want_h:
-        r.h = _empty2(M, F, torch.bfloat16, dev)
-        o.h = r.h.data_ptr()
-    if want_gu:
-        r.gu = _empty2(M, 2 * F, torch.bfloat16, dev)
-        o.gu = r.gu.data_ptr()
-    if want_amax:
-        r.amax = _amax_scalar(dev)
-        o.amax = r.amax.data_ptr()
-    if quantize_h:
-        c = r.quantized = _mxfp8_outputs(M, F, False, dev)
-        o.q, o.s, o.s_stride, o.s_swz = c.data.data_ptr(), c.scale.data_ptr(), F // 32, c.scale_swz.data_ptr()
+    r = GatedResult(_empty2(M, F, torch.bfloat16, dev) if want_h else None,
+                    _empty2(M, 2 * F, torch.bfloat16, dev) if want_gu else None,
+                    _mxfp8_outputs(M, F, False, dev) if quantize_h else None, _amax_scalar(dev) if want_amax else None)
+    c = r.quantized or _NO_COPIES
+    o = _lib.GatedOutputs(_ptr(r.h), _ptr(r.gu), _ptr(c.data), _ptr(c.scale), F // 32, _ptr(c.scale_swz), _ptr(r.amax))
     _count(1 if M and F else 0)
     if fmt == "mxfp8":
         _lib.call("mt_gemm_gated_mxfp8", qa.data_ptr(), sa_swz.data_ptr(), qb.data_ptr(), sb_swz.data_ptr(), _ptr(sb_up), M, F, K,
