@@ -31,7 +31,7 @@ constexpr int GG_SMEM = 8 * 3 * MX_TILE_BYTES + 128;
 // kDgu: the bf16 gradient or its abs-max is asked for; kCopies: the MXFP8 copies are. Spills cost more here than their
 // number says, since they queue behind the stores: one kernel for all of it, without the two __syncwarp that keep the
 // loads of a tile from being moved ahead all at once, spilled 22 registers and took 116 us instead of 110 on 4096 x
-// 14336 (copies), 226 instead of 204 on 8192 x 14336 (dgu alone).
+// 14336 (copies), 226 instead of 204 on 8192 x 14336 (dgu alone). Copies and gradient together still spill (28 registers).
 template <int kAct, bool kRagged, bool kDgu, bool kCopies>
 __global__ void __launch_bounds__(256, 2)
     gated_grad_kernel(const __grid_constant__ CUtensorMap map_dh, const __grid_constant__ CUtensorMap map_gu, const GatedGradArgs a) {
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(256, 2)
   }
   // padding of the GEMM-layout scales: beyond the last feature, and token blocks up to the padded count
   const int64_t mb0 = m0 >> 5, f1 = min(f0 + 128, a.F);
-  const bool last_x = tx == a.tiles_x - 1, last_y = tile >= a.tiles - a.tiles_x;
+  const bool last_x = tx == a.tiles_x - 1, last_y = (ty + 1) * a.tiles_x >= a.tiles;
   if (last_x) {
     mx_pad_row_scales(o, m0, 128, tid, 256);
     for (int i = 0; i < 4; ++i) mx_pad_col_features(o, mb0 + i, tid, 256);
