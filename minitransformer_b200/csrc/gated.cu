@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256, 2)
       wu[i][j] = f32x2_to_bf16x2(mul2(d2, act));
       wg[i][j] = f32x2_to_bf16x2(mul2(mul2(d2, bf16x2_to_f32x2(u[j])), grad));
     }
-    if (i % 4 == 3) __syncwarp();
+    if (kCopies ? i % 4 == 3 : i % 3 == 2) __syncwarp();   // (where nothing spills)
   }
   mx_release_tile(&empty[warp], ph, &abort_flag, a.status);
   if (lane == 0 && tile + (int)gridDim.x < a.tiles) fetch(tile + gridDim.x);

@@ -38,7 +38,15 @@ __device__ __forceinline__ float gated_act(float g) {
   return g * gated_sigmoid(2.0f * GELU_C * g * fmaf(GELU_A * g, g, 1.0f));
 }
 
-// act(g) and act'(g) of two values at once
+// The gate limited to +-16, where gelu's s (1 - s) has long vanished in fp32 (z = 318); a NaN stays one.
+__device__ __forceinline__ float gelu_limit(float g) {
+  float y;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(g), "f"(16.0f));
+  return y;
+}
+
+// act(g) and act'(g) of two values at once. gelu takes z and its slope, both cubic, of the limited gate: the slope of
+// the gate itself leaves fp32 beyond |g| = 1e13, and infinity times an s (1 - s) of zero is a NaN where act' is 0 or 1.
 template <int kAct>
 __device__ __forceinline__ void gated_act_grad2(f32x2_t g, f32x2_t& act, f32x2_t& grad) {
   const f32x2_t one = pack2(1.0f, 1.0f);
@@ -46,9 +54,12 @@ __device__ __forceinline__ void gated_act_grad2(f32x2_t g, f32x2_t& act, f32x2_t
   if (kAct == MT_ACT_SILU) {
     z = mul2(g, pack2(-LOG2E, -LOG2E));
   } else {
-    const f32x2_t gg = mul2(g, g);
-    z = mul2(mul2(g, pack2(-LOG2E * 2.0f * GELU_C, -LOG2E * 2.0f * GELU_C)), fma2(gg, pack2(GELU_A, GELU_A), one));
-    slope = mul2(mul2(g, pack2(2.0f * GELU_C, 2.0f * GELU_C)), fma2(gg, pack2(3.0f * GELU_A, 3.0f * GELU_A), one));
+    constexpr float C = 2.0f * GELU_C, CL = -LOG2E * 2.0f * GELU_C;
+    float g0, g1;
+    unpack2(g, g0, g1);
+    const f32x2_t gl = pack2(gelu_limit(g0), gelu_limit(g1)), gg = mul2(gl, gl);
+    z = mul2(gl, fma2(gg, pack2(CL * GELU_A, CL * GELU_A), pack2(CL, CL)));
+    slope = mul2(gl, fma2(gg, pack2(3.0f * C * GELU_A, 3.0f * C * GELU_A), pack2(C, C)));
   }
   float z0, z1, s0, s1;
   unpack2(z, z0, z1);

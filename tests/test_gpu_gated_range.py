@@ -1,0 +1,77 @@
+"""GPU tests of the gated projection and its gradient at the ends of their ranges.
+
+Tolerances count roundings: one to bf16 is off by at most 2^-8 of the value, an exponential of z by (1 + |z|) 2^-20 of
+its value (two fp32 steps of z, and the function's own error). A sigmoid below 2^-126 is a multiple of 2^-149 and so
+off by up to one such step on top; for |z| > 200 it is 0 or 1."""
+import math
+
+import pytest
+import torch
+
+from minitransformer_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+HALF, TINY, STEP = 2.0 ** -8, 2.0 ** -133, 2.0 ** -149
+
+
+def _rand(shape, seed, std=1.0, dtype=BF):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def _within(got, want, tol, what):
+    bad = ~((got.double() - want).abs() <= tol)          # (a NaN is not within anything)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off: {got[bad][:4].tolist()} for {want[bad][:4].tolist()}"
+
+
+def _same_copies(a, b, what):
+    for n in ("data", "scale", "scale_swz", "data_t", "scale_t", "scale_t_swz"):
+        x, y = getattr(a, n), getattr(b, n)
+        assert (x is None) == (y is None), (what, n)
+        if x is not None:
+            assert x.shape == y.shape and torch.equal(x.view(torch.uint8), y.view(torch.uint8)), (what, n)
+
+
+def _act64(g, act):
+    """act, act', the sigmoid inside, the slope of its argument times g (what act' multiplies s (1 - s) by), its argument."""
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s)), s, g, g
+    c, a = math.sqrt(2 / math.pi), 0.044715
+    z = 2 * c * (g + a * g ** 3)
+    s = torch.sigmoid(z)
+    slope = 2 * g * c * (1 + 3 * a * g * g)
+    return g * s, s + slope * s * (1 - s), s, slope, z
+
+
+def _check_gradient(dh, gu, act):
+    r = K.gated_backward(dh, gu, activation=act, want_dgu=True, want_amax=True)
+    g, u = gu.double().split(dh.shape[1], 1)
+    a, d, s, slope, z = _act64(g, act)
+    D = dh.double()
+    soft = (1 + z.abs().clamp(max=200)) * 2.0 ** -20     # beyond, the sigmoid is 0 or 1
+    # act' = s + slope s (1 - s): the magnitudes of both terms, where the second has not vanished
+    terms = s + torch.where(s * (1 - s) > 0, (d - s).abs(), torch.zeros_like(s))
+    reach = torch.where(z.abs() < 200, 1 + slope.abs(), torch.ones_like(s))
+    want = torch.cat([D * u * d, D * a], 1)
+    tol = torch.cat([HALF * (D * u * d).abs() + soft * (D * u).abs() * terms + (D * u).abs() * reach * STEP,
+                     (HALF + torch.where(z.abs() < 200, soft, torch.zeros_like(s))) * (D * a).abs() + D.abs() * (g.abs().clamp(max=200) + 1) * STEP], 1)
+    _within(r.dgu, want, tol + TINY, f"dgu {act}")
+    _same_copies(r.quantized, K.quantize_mxfp8(r.dgu), "gradient")
+    _same_copies(K.gated_backward(dh, gu, activation=act).quantized, r.quantized, "alone")
+    assert float(r.amax) == float(r.dgu.abs().max().float())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows", [32, 9])
+def test_gated_gradient_of_huge_gates(act, rows):
+    """Gates up to the largest bf16 value: the derivative is 1 or 0 there, never a NaN, with dh of 0 as well."""
+    F = 64
+    g = torch.tensor([s * v for v in (16.5, 1e3, 1e9, 1e13, 1.3e13, 1e15, 1e19, 3e19, 1e30, 3.3e38) for s in (1, -1)], device="cuda").to(BF)
+    gu, dh = _rand((rows, 2 * F), 1), _rand((rows, F), 2, 1e-2)
+    gu[1, :20], gu[4, 30:50], gu[rows - 1, 44:64] = g, g, g
+    dh[4, 30:50] = 0
+    _check_gradient(dh, gu, act)
+    r = K.gated_backward(dh, gu, activation=act, want_dgu=True)
+    assert not bool(r.dgu[4, 30:50].any()) and not bool(r.dgu[4, F + 30:F + 50].any())
