@@ -75,3 +75,56 @@ def test_gated_gradient_of_huge_gates(act, rows):
     _check_gradient(dh, gu, act)
     r = K.gated_backward(dh, gu, activation=act, want_dgu=True)
     assert not bool(r.dgu[4, 30:50].any()) and not bool(r.dgu[4, F + 30:F + 50].any())
+
+
+def _gates(x0, w0, up):
+    """Operands whose gates are exactly x0[i] * w0[j] and whose second projection is `up`: one non-zero column each, in
+    blocks of their own (x0, w0 and up on the E4M3 grid up to powers of two). Features beyond w0 have a gate of zero; with
+    many rows there are enough of them for the kernel of 256-row pairs."""
+    M, F, Kd = len(x0), 32 if len(x0) < 256 else 4096, 64
+    x, w = torch.zeros(M, Kd, dtype=BF, device="cuda"), torch.zeros(2 * F, Kd, dtype=BF, device="cuda")
+    x[:, 0], x[:, 32] = torch.tensor(x0, device="cuda").to(BF), 1.0
+    w[:len(w0), 0], w[F:, 32] = torch.tensor(w0, device="cuda").to(BF), up
+    q = [K.quantize_mxfp8(t, return_transpose=False) for t in (x, w)]
+    g = x[:, :1].double() * w[None, :F, 0].double()
+    return q, g, F
+
+
+def _check_projection(x0, w0, up, act, M):
+    (qx, qw), g, F = _gates((x0 * M)[:M], w0, up)
+    r = K.gemm_gated_mxfp8(qx.data, qx.scale_swz, qw.data, qw.scale_swz, activation=act, sb_lin=qw.scale, want_gu=True,
+                           quantize_h=True, want_amax=True)
+    assert torch.equal(r.gu[:, :F].double(), g.to(BF).double()) and bool((r.gu[:, F:].double() == up).all())
+    a, d, s, slope, z = _act64(g, act)
+    soft = torch.where(z.abs() < 200, (1 + z.abs()) * 2.0 ** -20, torch.zeros_like(z))
+    want = a * up
+    _within(r.h, want, (HALF + soft) * want.abs() + (g.abs().clamp(max=200) + 1) * abs(up) * STEP + TINY, f"h {act}")
+    _same_copies(r.quantized, K.quantize_mxfp8(r.h, return_transpose=False), "projection")
+    assert float(r.amax) == float(r.h.abs().max().float())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M", [12, 300])
+def test_gated_projection_of_huge_gates(act, M):
+    x0 = [s * 2.0 ** p for p in (0, 20, 44, 50, 63) for s in (1.0, -1.75)]
+    _check_projection(x0, [2.0 ** p for p in (0, 3, 20, 40, 60, 62)], 0.5, act, M)
+
+
+@pytest.mark.parametrize("act,values", [("silu", [80.0, 88.0, 96.0, 104.0]), ("gelu", [7.0, 9.0, 10.0, 11.0])])
+@pytest.mark.parametrize("up", [1.5, 2.0 ** 40])
+@pytest.mark.parametrize("M", [8, 300])
+def test_gated_projection_where_the_sigmoid_is_subnormal(act, values, up, M):
+    _check_projection([-v for v in values] + values, [1.0, 1.125, 1.25, 1.5, 0.875], up, act, M)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 40])
+def test_gated_gradient_where_the_sigmoid_is_subnormal(act, scale):
+    """Gates whose sigmoid lies below the smallest normal fp32 value, and those at the root of act'."""
+    g = {"silu": [-85, -87, -87.5, -88, -88.5, -89, -90, -92, -96, -100, -103, -104, -110, -200, -1.28125],
+         "gelu": [-9.5, -9.9375, -10, -10.0625, -10.125, -10.25, -10.5, -10.75, -11, -12, -14, -20, -0.75390625]}[act]
+    gu, dh = _rand((64, 128), 1), _rand((64, 64), 2)
+    gu[7, :len(g)] = torch.tensor(g, device="cuda").to(BF)
+    gu[:, 64:] = 1.5
+    dh[7] = scale
+    _check_gradient(dh, gu, act)
