@@ -145,7 +145,7 @@ class GatedLinear(LayerLinearBaseModule):
     own [gate shard; up shard]). Other arguments as in `Linear`.
 
     emit_quantized (attribute, off by default): `output_meta` holds what the next layer's quantizer can
-    take over for h, to be given as its `inp_meta`: the row-wise MXFP8 copy (used by a forward pass
+    take over for h, to be given as its `inp_meta`: the row-wise MXFP8 copy, as long as h lives (used by a forward pass
     without gradients; a training pass also needs a transposed copy and quantizes h itself), or max |h|
     under an NVFP4 recipe."""
 
@@ -207,4 +207,7 @@ class GatedLinear(LayerLinearBaseModule):
         args = (inp, inp_meta, self.weight, self.weight_qresult_cache, self.activation, self.tp_group, self.tp_size,
                 self.parallel_mode, self.qlinear_params, self.activation_dtype, grad, is_first_microbatch,
                 self.fuse_wgrad_accumulation, out_meta)
-        return _QuantizedGatedLinear.apply(*args) if grad else _QuantizedGatedLinear.forward(None, *args)
+        h = _QuantizedGatedLinear.apply(*args) if grad else _QuantizedGatedLinear.forward(None, *args)
+        if out_meta is not None and out_meta[0].quantized is not None:
+            out_meta[0].quantized = quantization.TensorCopies(h, out_meta[0].quantized)
+        return h

@@ -55,7 +55,7 @@ class RMSNorm(torch.nn.Module):
     copies) up to 32768, weight in bf16 or fp32.
 
     emit_quantized (attribute, off by default): `output_meta` holds what the recipe's quantizer can take
-    over for y, for the next layer's `inp_meta`. qlinear_params: that layer's recipe; if None it is
+    over for y, for the next layer's `inp_meta`; MXFP8 copies live as long as the y they belong to. qlinear_params: that layer's recipe; if None it is
     taken from QAT_PARAMS the first time it is needed."""
 
     def __init__(self, hidden_size: int, eps: float = 1e-5, params_dtype: Optional[torch.dtype] = None, device="cuda",
@@ -85,5 +85,9 @@ class RMSNorm(torch.nn.Module):
         self.output_meta = quantization.QuantizeInputMeta() if copies else None
         grad = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or
                                             (residual is not None and residual.requires_grad))
-        args = (x, residual, self.weight, self.eps, copies, grad, self.output_meta)
-        return _RMSNorm.apply(*args) if grad else _RMSNorm.forward(None, *args)
+        meta = self.output_meta
+        args = (x, residual, self.weight, self.eps, copies, grad, meta)
+        out = _RMSNorm.apply(*args) if grad else _RMSNorm.forward(None, *args)
+        if meta is not None and meta.quantized is not None:
+            meta.quantized = quantization.TensorCopies(out if residual is None else out[0], meta.quantized)
+        return out

@@ -39,9 +39,13 @@ class Mxfp8QuantizeOp(Q.QuantizeOpBase):
         x = _as_2d_bf16(x)
         into = getattr(input_meta, "into", None)
         made = getattr(input_meta, "quantized", None)
+        if made is not None:
+            held = made.shape if isinstance(made, Q.TensorCopies) else tuple(made.data.shape)
+            if into is None and held != tuple(x.shape):
+                raise kernels._lib.MtError(f"copies of a {held} tensor given for one of shape {tuple(x.shape)}")
+            if isinstance(made, Q.TensorCopies):
+                made = made.of(x)
         if made is not None and into is None and (made.data_t is not None or not return_transpose):
-            if tuple(made.data.shape) != tuple(x.shape):
-                raise kernels._lib.MtError(f"copies of a {tuple(made.data.shape)} tensor given for one of shape {tuple(x.shape)}")
             return made
         r = kernels.quantize_mxfp8(x, return_transpose=return_transpose, into=into)
         return as_quantize_result(r)

@@ -6,7 +6,8 @@ its `quantize` and `qgemm`. Names, fields and argument meaning are kept so that 
 recipes and callers keep working; the implementations behind them are the sm_100a kernels.
 """
 import dataclasses
-from typing import Optional, Tuple
+import weakref
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -102,6 +103,30 @@ class QuantizeResultCache:
                 getattr(self, lin)._mt_swz = getattr(self, swz)
 
 
+class TensorCopies:
+    """Quantized copies that the producer of a tensor made along with it. They hang on that tensor and go when it does,
+    so that a module which remembers this object keeps no memory alive."""
+
+    def __init__(self, tensor: torch.Tensor, copies: QuantizeResult) -> None:
+        tensor._mt_copies = copies
+        self.shape = tuple(copies.data.shape)
+        self._tensor = weakref.ref(tensor)
+
+    def of(self, x: torch.Tensor) -> Optional[QuantizeResult]:
+        """The copies, if their tensor is still there, else None."""
+        tensor = self._tensor()
+        return None if tensor is None else tensor._mt_copies
+
+    def __reduce__(self):
+        return _gone_copies, (self.shape,)       # a copied or unpickled module remembers no tensor
+
+
+def _gone_copies(shape) -> TensorCopies:
+    c = TensorCopies.__new__(TensorCopies)
+    c.shape, c._tensor = shape, (lambda: None)
+    return c
+
+
 @dataclasses.dataclass
 class QuantizeInputMetaBase:
     """Side information about a quantize input (e.g. an abs-max computed by the producer)."""
@@ -125,13 +150,14 @@ class QuantizeInputMeta(QuantizeInputMetaBase):
         col_sum_done when it has filled it (formats without an abs-max pass leave it alone).
     quantized: the copies of exactly this tensor, made by its producer (RMSNorm or GatedLinear with
         emit_quantized); the MXFP8 quantizer returns them instead of reading the tensor again,
-        where they hold what the call needs (the transposed copy too when that is asked for)."""
+        where they hold what the call needs (the transposed copy too when that is asked for). The
+        layers give TensorCopies, which leave the copies with their tensor."""
     amax_col: Optional[torch.Tensor] = None
     into: Optional[dict] = None
     amax_reduce: Optional[object] = None
     col_sum: Optional[torch.Tensor] = None
     col_sum_done: bool = False
-    quantized: Optional[QuantizeResult] = None
+    quantized: Union[QuantizeResult, TensorCopies, None] = None
 
 
 class QuantizeOpBase:
