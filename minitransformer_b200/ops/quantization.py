@@ -105,17 +105,23 @@ class QuantizeResultCache:
 
 class TensorCopies:
     """Quantized copies that the producer of a tensor made along with it. They hang on that tensor and go when it does,
-    so that a module which remembers this object keeps no memory alive."""
+    so that a module which remembers this object keeps no memory alive, and they count for that tensor alone, as long
+    as it has not been changed in place (changes made in inference mode go unnoticed: torch does not count them)."""
 
     def __init__(self, tensor: torch.Tensor, copies: QuantizeResult) -> None:
         tensor._mt_copies = copies
         self.shape = tuple(copies.data.shape)
         self._tensor = weakref.ref(tensor)
+        self._version = None if tensor.is_inference() else tensor._version
 
     def of(self, x: torch.Tensor) -> Optional[QuantizeResult]:
-        """The copies, if their tensor is still there, else None."""
+        """The copies, if the matrix x is that tensor as it was (its memory cannot be another's while it lives), else None."""
         tensor = self._tensor()
-        return None if tensor is None else tensor._mt_copies
+        if tensor is None or tensor.data_ptr() != x.data_ptr():
+            return None
+        if self._version is not None and tensor._version != self._version:
+            return None
+        return tensor._mt_copies
 
     def __reduce__(self):
         return _gone_copies, (self.shape,)       # a copied or unpickled module remembers no tensor
@@ -123,7 +129,7 @@ class TensorCopies:
 
 def _gone_copies(shape) -> TensorCopies:
     c = TensorCopies.__new__(TensorCopies)
-    c.shape, c._tensor = shape, (lambda: None)
+    c.shape, c._tensor, c._version = shape, (lambda: None), None
     return c
 
 

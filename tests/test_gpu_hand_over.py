@@ -1,8 +1,9 @@
-"""GPU tests of what the norm and the gated projection hand on to the next layer: memory, and who takes it."""
+"""GPU tests of what the norm and the gated projection hand on to the next layer: memory, who takes it, and inputs changed in between."""
 import pytest
 import torch
 
 from minitransformer_b200.module import config
+from minitransformer_b200.module.gated_linear import GatedLinear
 from minitransformer_b200.module.linear import Linear
 from minitransformer_b200.module.rmsnorm import RMSNorm
 
@@ -54,6 +55,23 @@ def test_copies_do_not_outlive_the_tensor_they_belong_to():
             forward()
         held[emit] = (after_forward, after_backward, torch.cuda.memory_allocated() - base)
     assert all(a <= b for a, b in zip(held[True], held[False])), held
+
+
+def test_copies_of_a_changed_tensor_are_not_used():
+    norm = RMSNorm(256, params_dtype=BF, qlinear_params=MXFP8)
+    norm.emit_quantized = True
+    lin = Linear(256, 128, bias=False, params_dtype=BF, qlinear_params=MXFP8)
+    gated = GatedLinear(256, 128, params_dtype=BF, qlinear_params=MXFP8)
+    x = _rand((64, 256), 1)
+    with torch.no_grad():
+        for layer in (lin, gated):
+            y = norm(x)
+            same = layer(y, inp_meta=norm.output_meta)
+            assert torch.equal(same, layer(y.clone()))
+            y.mul_(-3)
+            assert torch.equal(layer(y, inp_meta=norm.output_meta), layer(y.clone()))
+            other = _rand((64, 256), 9)
+            assert torch.equal(layer(other, inp_meta=norm.output_meta), layer(other))
 
 
 def test_one_norm_feeds_several_layers_from_its_copies():

@@ -31,6 +31,17 @@ def test_copies_live_as_long_as_their_tensor():
     assert alive() is None and t.of(torch.zeros(32, 64, dtype=torch.bfloat16)) is None
 
 
+def test_copies_count_for_their_tensor_unchanged():
+    y, made = torch.zeros(32, 64, dtype=torch.bfloat16), _copies(32, 64)
+    t = Q.TensorCopies(y, made)
+    assert t.of(y.detach().reshape(32, 64)) is made and t.of(y.clone()) is None
+    y[3].add_(1)
+    assert t.of(y) is None
+    with torch.inference_mode():
+        z = torch.zeros(32, 64, dtype=torch.bfloat16)
+        assert Q.TensorCopies(z, made).of(z) is made
+
+
 def test_a_copied_or_pickled_holder_remembers_no_tensor():
     y = torch.zeros(32, 64, dtype=torch.bfloat16)
     t = Q.TensorCopies(y, _copies(32, 64))
@@ -53,6 +64,10 @@ def test_the_quantizer_takes_copies_only_where_they_hold(monkeypatch):
     assert op.quantize(y, p, input_meta=meta) is made and not calls
     assert op.quantize(y.view(2, 16, 64), p, input_meta=meta) is made and not calls
     assert op.quantize(y, p, return_transpose=True, input_meta=meta).data_t is not None and calls == [True]
+    op.quantize(y.clone(), p, input_meta=meta)                  # equal, but not that tensor: read again
+    y.mul_(2)
+    op.quantize(y, p, input_meta=meta)
+    assert calls == [True, False, False]
     with pytest.raises(_lib.MtError, match="copies of"):
         op.quantize(y[:16], p, input_meta=meta)
     # a caller's own result counts as given
