@@ -16,7 +16,7 @@ import torch
 
 from . import config
 from .base import LayerLinearBaseModule
-from .linear import _QuantizedLinear
+from .linear import _overlap_sm_margin, _QuantizedLinear, _sm_margin
 from .. import kernels
 from ..distributed.distributed import allreduce, set_tensor_model_parallel_attributes
 from ..ops import quantization
@@ -105,10 +105,12 @@ class _QuantizedGatedLinear(torch.autograd.Function):
         if w.requires_grad:
             accumulate = ctx.fuse_wgrad_accumulation and (ctx.is_first_microbatch is None or not ctx.is_first_microbatch)
             main_grad = w.main_grad if ctx.fuse_wgrad_accumulation else None
-            wgrad = op.qgemm(qres_d.data_t, qx_t, p.mm_wgrad,
-                             main_grad.dtype if main_grad is not None else (p.mm_wgrad.out_dtype or w.dtype), qres_d.scale_t,
-                             sx_t, None, out=main_grad, accumulate=accumulate, global_amax_qx=qres_d.global_amax_col,
-                             global_amax_qw=amax_x_col, qparams_x=p.g_params, qparams_w=p.x_params)
+            # an all-reduce of dgrad is in flight: leave it SMs to run on
+            with _sm_margin(op, _overlap_sm_margin() if handle is not None else 0):
+                wgrad = op.qgemm(qres_d.data_t, qx_t, p.mm_wgrad,
+                                 main_grad.dtype if main_grad is not None else (p.mm_wgrad.out_dtype or w.dtype), qres_d.scale_t,
+                                 sx_t, None, out=main_grad, accumulate=accumulate, global_amax_qx=qres_d.global_amax_col,
+                                 global_amax_qw=amax_x_col, qparams_x=p.g_params, qparams_w=p.x_params)
             wgrad = _QuantizedLinear.reset_wgrad_if_needed(ctx, w, wgrad)
         if handle is not None:
             handle.wait()
