@@ -162,6 +162,8 @@ class GatedLinear(LayerLinearBaseModule):
         if parallel_mode not in ("column", None):
             raise kernels._lib.MtError(f"GatedLinear: parallel_mode {parallel_mode!r} is not supported (None or 'column')")
         params_dtype = torch.get_default_dtype() if params_dtype is None else params_dtype
+        if self.tp_size > 1 and torch.cuda.is_available():
+            kernels.set_launch_overlap(False)      # as Linear does: kernels resident early would take the SMs of the exchanges
         self.in_features, self.activation, self.parallel_mode = in_features, activation, parallel_mode
         self.ffn_size = divide(ffn_size, self.tp_size) if parallel_mode == "column" else ffn_size
         if self.in_features % 32 or self.ffn_size % 32:

@@ -4,6 +4,7 @@ import contextlib
 import pytest
 import torch
 
+from minitransformer_b200 import kernels
 from minitransformer_b200.module import config, gated_linear
 from test_norm_gated_cpu import _ExactOp
 
@@ -43,3 +44,13 @@ def test_wgrad_leaves_sms_to_the_all_reduce_of_dgrad(monkeypatch, tp_size, margi
     x = torch.randn(32, 32).to(torch.bfloat16).requires_grad_()
     lin(x).sum().backward()
     assert op.seen == margins and x.grad is not None and lin.weight.grad is not None
+
+
+@pytest.mark.parametrize("tp_size,switched", [(1, []), (2, [False])])
+def test_tensor_parallel_layers_switch_early_launches_off(monkeypatch, tp_size, switched):
+    calls = []
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(kernels, "set_launch_overlap", calls.append)
+    gated_linear.GatedLinear(32, 64, parallel_mode="column", tp_size=tp_size, device="meta", params_dtype=torch.bfloat16,
+                             qlinear_params=config.QLinearParams(quantize=True, quantize_op=_MarginOp()))
+    assert calls == switched
