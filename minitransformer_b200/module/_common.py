@@ -1,9 +1,21 @@
 """Concatenation of parameter views that avoids a copy when the views already sit back to
-back in one buffer (what `parameters_split` creates). Same role as
-miniTransformer/module/_common.py:98-113."""
-from typing import Sequence
+back in one buffer (what `parameters_split` creates; same role as
+miniTransformer/module/_common.py:98-113), and the refusal of derivatives that a layer has none of."""
+from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
+
+from .._lib import MtError
+
+
+def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises where an input carries a forward-mode tangent: the kernels would lose it in silence."""
+    if forward_ad._current_level < 0:            # outside of any dual level: no tensor has one
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise MtError(f"{what}: forward-mode derivatives are not implemented")
 
 
 class _NoopCat(torch.autograd.Function):

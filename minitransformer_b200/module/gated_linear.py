@@ -15,6 +15,7 @@ from typing import Callable, Optional, Union
 import torch
 
 from . import config
+from ._common import refuse_tangents
 from .base import LayerLinearBaseModule
 from .linear import _overlap_sm_margin, _QuantizedLinear, _sm_margin
 from .. import kernels
@@ -134,6 +135,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, *, activation: str = "si
     params = config.get_qlinear_params_from_env_qat_params() if qlinear_params is None else qlinear_params
     if not params.quantize:
         return _non_quantized(x, weight, activation)
+    refuse_tangents("gated_linear", x, weight)
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
     args = (x, inp_meta, weight, None, activation, None, 1, None, params, x.dtype, grad, None,
             False, None)
@@ -201,6 +203,7 @@ class GatedLinear(LayerLinearBaseModule):
             if self.parallel_mode == "column" and self.tp_size > 1:
                 raise kernels._lib.MtError("GatedLinear: tensor parallelism needs a quantized recipe")
             return _non_quantized(inp, self.weight, self.activation)
+        refuse_tangents("GatedLinear", inp, self.weight)
         self.weight_qresult_cache.keep = bool(self.primary_weights_in_fp8)
         grad = torch.is_grad_enabled()
         out_meta = None

@@ -10,6 +10,7 @@ from typing import Optional
 import torch
 
 from . import config
+from ._common import refuse_tangents
 from .. import kernels
 from ..ops import quantization
 from ..ops.mxfp8_quantize_op import Mxfp8QuantizeOp, as_quantize_result
@@ -81,6 +82,7 @@ class RMSNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
         if residual is not None and residual.shape != x.shape:
             raise kernels._lib.MtError(f"residual of shape {tuple(residual.shape)} for x of shape {tuple(x.shape)}")
+        refuse_tangents("RMSNorm", x, residual, self.weight)
         copies = self._copies()
         self.output_meta = quantization.QuantizeInputMeta() if copies else None
         grad = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or
