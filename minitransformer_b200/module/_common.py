@@ -1,6 +1,7 @@
 """Concatenation of parameter views that avoids a copy when the views already sit back to
 back in one buffer (what `parameters_split` creates; same role as
 miniTransformer/module/_common.py:98-113), and the refusal of derivatives that a layer has none of."""
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -16,6 +17,40 @@ def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise MtError(f"{what}: forward-mode derivatives are not implemented")
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """Its inputs, with a gradient that is an error."""
+
+    @staticmethod
+    def forward(ctx, what, *grads):
+        ctx.what = what
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise MtError(f"{ctx.what}: second derivatives are not implemented")
+
+
+def first_derivatives_only(what: str):
+    """Decorator of an autograd function's backward whose kernels autograd cannot see into: with create_graph its results
+    depend on the inputs and on the incoming gradient, and differentiating them raises instead of leaving that out."""
+    def decorate(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *grads)
+            with torch.no_grad():
+                out = list(backward(ctx, *grads))
+            # (an incoming gradient handed through keeps what it depends on)
+            at = [i for i, t in enumerate(out) if t is not None and not any(t is g for g in grads)]
+            if not at:
+                return tuple(out)
+            for i, t in zip(at, _NoSecondDerivative.apply(what, *(out[i].detach().requires_grad_() for i in at))):
+                out[i] = t
+            return tuple(out)
+        return run
+    return decorate
 
 
 class _NoopCat(torch.autograd.Function):

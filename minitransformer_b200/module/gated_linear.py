@@ -15,7 +15,7 @@ from typing import Callable, Optional, Union
 import torch
 
 from . import config
-from ._common import refuse_tangents
+from ._common import first_derivatives_only, refuse_tangents
 from .base import LayerLinearBaseModule
 from .linear import _overlap_sm_margin, _QuantizedLinear, _sm_margin
 from .. import kernels
@@ -82,6 +82,7 @@ class _QuantizedGatedLinear(torch.autograd.Function):
         return r.h[:M].view(*x_shape[:-1], r.h.shape[-1])
 
     @staticmethod
+    @first_derivatives_only("GatedLinear")
     def backward(ctx, dh):
         qx_t, sx_t, amax_x_col, qw_t, sw_t, amax_w_col, gu, w = ctx.saved_tensors
         p, op = ctx.qlinear_params, ctx.quantize_op

@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import config
-from ._common import refuse_tangents
+from ._common import first_derivatives_only, refuse_tangents
 from .. import kernels
 from ..ops import quantization
 from ..ops.mxfp8_quantize_op import Mxfp8QuantizeOp, as_quantize_result
@@ -39,6 +39,7 @@ class _RMSNorm(torch.autograd.Function):
         return y if residual is None else (y, r.h.view(shape))
 
     @staticmethod
+    @first_derivatives_only("RMSNorm")
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
         cols = ctx.shape[-1]

@@ -44,3 +44,23 @@ def test_forward_mode_tangents_are_refused(norm, grad):
         # without a tangent, and where torch computes, the level changes nothing
         norm(x, r), lin(x)
         assert forward_ad.unpack_dual(gated_linear(dx, w, qlinear_params=PLAIN)).tangent is not None
+
+
+def test_second_derivatives_are_refused(norm):
+    x, r = torch.randn(32, 32).to(BF).requires_grad_(), torch.randn(32, 32).to(BF).requires_grad_()
+    lin = GatedLinear(32, 32, device="cpu", params_dtype=BF, qlinear_params=EXACT)
+    for f, inputs in ((lambda: norm(x), (x, norm.weight)), (lambda: sum(norm(x, r)), (x, r)), (lambda: lin(x), (x, lin.weight))):
+        y = f()
+        once = torch.autograd.grad(y.sum(), inputs, retain_graph=True)
+        first = torch.autograd.grad(y.sum(), inputs, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(once, first))
+        with pytest.raises(_lib.MtError, match="second derivatives"):
+            (y.sum() + sum(g.square().sum() for g in first)).backward()
+    # gradients that are not differentiated again may have been taken with create_graph
+    lin(x).sum().backward(create_graph=True)
+    assert x.grad is not None and lin.weight.grad is not None
+    # the residual stream alone is an addition, with all its derivatives
+    x.grad = None
+    first, = torch.autograd.grad(norm(x, r)[1].square().sum(), x, create_graph=True)
+    first.sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 2))
