@@ -125,6 +125,7 @@ def _non_quantized(x, w, activation):
     return a * u
 
 
+@torch._dynamo.disable(recursive=True)
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, *, activation: str = "silu",
                  qlinear_params: Optional[config.QLinearParams] = None,
                  inp_meta: Optional[quantization.QuantizeInputMetaBase] = None) -> torch.Tensor:
