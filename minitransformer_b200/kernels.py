@@ -258,7 +258,7 @@ def gemm_options(sm_margin: Optional[int] = None, d_amax: Optional[torch.Tensor]
     runs beside it instead of behind it; d_amax: fp32 device scalar (zeroed by the caller) that
     the GEMM raises to the largest |value| it stores; scatter = (addresses of the ranks' staging
     buffers, this rank, rows per rank): the output rows go to the ranks' staging buffers instead
-    of an output tensor (the GEMM call then returns None)."""
+    of an output tensor (the GEMM call then returns None). The gated projections take no margin and refuse the others."""
     prev = getattr(_GEMM_OPTS, "value", None)
     base = prev or (0, None, None)     # nested contexts inherit what they do not set
     _GEMM_OPTS.value = (base[0] if sm_margin is None else int(sm_margin), base[1] if d_amax is None else d_amax,
@@ -696,6 +696,9 @@ class GatedResult:
 
 
 def _gemm_gated(fmt, qa, sa_swz, amax_a, qb, sb_swz, amax_b, activation, sb_lin, want_h, want_gu, quantize_h, want_amax):
+    options = getattr(_GEMM_OPTS, "value", None)
+    if options is not None and (options[1] is not None or options[2] is not None):
+        raise _lib.MtError("gated projection: gemm_options(d_amax=..., scatter=...) are those of the plain GEMMs (want_amax gives max |h|)")
     _same_device(qa, sa_swz=sa_swz, qb=qb, sb_swz=sb_swz, amax_a=amax_a, amax_b=amax_b, sb_lin=sb_lin)
     act = _activation_code(activation)
     if qa.dim() != 2 or qb.dim() != 2 or qa.shape[1] != qb.shape[1] or qb.shape[0] % 2:
