@@ -128,3 +128,41 @@ def test_gated_gradient_where_the_sigmoid_is_subnormal(act, scale):
     gu[:, 64:] = 1.5
     dh[7] = scale
     _check_gradient(dh, gu, act)
+
+
+def test_infinities_and_nan_reach_the_projection():
+    """NaN codes and infinite projections: h is NaN or infinite where the formula is, its copies are the quantize kernel's."""
+    for M, F in ((40, 96), (300, 4096)):
+        for act in ("silu", "gelu"):
+            x, w = _rand((M, 64), 1), _rand((2 * F, 64), 2, 0.05)
+            qx, qw = (K.quantize_mxfp8(t, return_transpose=False) for t in (x, w))
+            clean = K.gemm_gated_mxfp8(qx.data, qx.scale_swz, qw.data, qw.scale_swz, activation=act, sb_lin=qw.scale, quantize_h=True)
+            qx.data[3, 5] = 0x7F                                   # a NaN among the inputs
+            qw.data[9, 7] = 0x7F                                   # ... and in a gate's weights
+            r = K.gemm_gated_mxfp8(qx.data, qx.scale_swz, qw.data, qw.scale_swz, activation=act, sb_lin=qw.scale, quantize_h=True, want_amax=True)
+            bad = torch.isnan(r.h)
+            want = torch.zeros_like(bad)
+            want[3], want[:, 9] = True, True
+            assert torch.equal(bad, want) and torch.equal(r.h[~bad], clean.h[~bad])
+            _same_copies(r.quantized, K.quantize_mxfp8(r.h, return_transpose=False), "nan")
+            assert float(r.amax) == float(r.h[~bad].abs().max().float())
+    # infinite projections: 2^100 * 2^100, and a second projection of both signs
+    for M in (8, 300):
+        x0 = ([2.0 ** 100, -2.0 ** 100, 1.0, 0.0] * M)[:M]
+        for act in ("silu", "gelu"):
+            (qx, qw), g, F = _gates(x0, [2.0 ** 100, 1.0, -2.0 ** 100], 2.0)
+            r = K.gemm_gated_mxfp8(qx.data, qx.scale_swz, qw.data, qw.scale_swz, activation=act, sb_lin=qw.scale, want_gu=True, quantize_h=True)
+            assert bool((r.h[0::4, 0] == float("inf")).all()) and bool((r.h[1::4, 2] == float("inf")).all())
+            assert bool(torch.isnan(r.h[0::4, 2]).all())           # -inf * 0, as the formula has it
+            assert bool((r.h[3::4] == 0).all())
+            _same_copies(r.quantized, K.quantize_mxfp8(r.h, return_transpose=False), "inf")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_infinities_and_nan_in_the_gradient(act):
+    gu, dh = _rand((96, 256), 2), _rand((96, 128), 3)
+    gu[1, 3], gu[40, 128 + 5], dh[70, 9] = float("nan"), float("inf"), float("nan")
+    r = K.gated_backward(dh, gu, activation=act, want_dgu=True)
+    bad = ~torch.isfinite(r.dgu)
+    assert bool(bad[1, 3]) and bool(bad[1, 131]) and bool(bad[40, 5]) and bool(bad[70, 9]) and bool(bad[70, 137]) and int(bad.sum()) == 5
+    _same_copies(r.quantized, K.quantize_mxfp8(r.dgu), "inf")
