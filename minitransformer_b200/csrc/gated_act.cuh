@@ -75,7 +75,7 @@ __device__ __forceinline__ void gated_act_grad2(f32x2_t g, f32x2_t& act, f32x2_t
   unpack2(fma2(t, t, unit), s0, s1);
   const f32x2_t s = mul2(pack2(rcp_approx(s0), rcp_approx(s1)), unit);
   act = mul2(g, s);
-  grad = fma2(kAct == MT_ACT_SILU ? act : mul2(slope, s), sub2(one, s), s);   // s + slope s (1 - s)
+  grad = mul2(s, fma2(slope, sub2(one, s), one));   // s + slope s (1 - s)
 }
 
 #endif  // __CUDACC__
