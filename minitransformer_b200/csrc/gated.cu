@@ -65,99 +65,99 @@ __global__ void __launch_bounds__(256, 2)
   if (lane == 0 && (int)blockIdx.x < a.tiles) fetch(blockIdx.x);
   uint32_t ph = 0;
   for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ph ^= 1) {
-  const int ty = tile / a.tiles_x, tx = tile - ty * a.tiles_x;
-  const int64_t m0 = (int64_t)ty * 128, f0 = (int64_t)tx * 128;
-  const int64_t row0 = m0 + wr * 32, c0 = f0 + wc * 64;
-  uint8_t (&s_row)[2][128][4] = s_rows[ph], (&s_col)[2][128][4] = s_cols[ph];   // turns alternate: one barrier each
-  // on expiry the status word tells; the warp goes on with what is there, so that nobody waits for it
-  mbar_wait_bounded(&bars[warp], ph, &abort_flag, a.status, DS_QUANT_WAIT);
-  uint32_t wg[8][4], wu[8][4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4 g4 = mx_tile_row(buf, i), d4 = mx_tile_row(buf + MX_TILE_BYTES, i), u4 = mx_tile_row(buf + 2 * MX_TILE_BYTES, i);
-    const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f32x2_t act, grad;
-      gated_act_grad2<kAct>(bf16x2_to_f32x2(g[j]), act, grad);
-      const f32x2_t d2 = bf16x2_to_f32x2(d[j]);
-      wu[i][j] = f32x2_to_bf16x2(mul2(d2, act));
-      wg[i][j] = f32x2_to_bf16x2(mul2(mul2(d2, bf16x2_to_f32x2(u[j])), grad));
-    }
-    if (kCopies ? i % 4 == 3 : i % 3 == 2) __syncwarp();   // (where nothing spills)
-  }
-  mx_release_tile(&empty[warp], ph, &abort_flag, a.status);
-  if (lane == 0 && tile + (int)gridDim.x < a.tiles) fetch(tile + gridDim.x);
-  if (kDgu && a.dgu != nullptr) {
-    const int64_t row = row0 + (lane >> 3) * 8, f = c0 + (lane & 7) * 8;
-    const int nrow = f < a.F ? mx_valid_rows(a.rows, row) : 0;
-    __nv_bfloat16* pg = a.dgu + row * 2 * a.F + f;
+    const int ty = tile / a.tiles_x, tx = tile - ty * a.tiles_x;
+    const int64_t m0 = (int64_t)ty * 128, f0 = (int64_t)tx * 128;
+    const int64_t row0 = m0 + wr * 32, c0 = f0 + wc * 64;
+    uint8_t (&s_row)[2][128][4] = s_rows[ph], (&s_col)[2][128][4] = s_cols[ph];   // turns alternate: one barrier each
+    // on expiry the status word tells; the warp goes on with what is there, so that nobody waits for it
+    mbar_wait_bounded(&bars[warp], ph, &abort_flag, a.status, DS_QUANT_WAIT);
+    uint32_t wg[8][4], wu[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < nrow) {
-        *reinterpret_cast<uint4*>(pg) = make_uint4(wg[i][0], wg[i][1], wg[i][2], wg[i][3]);
-        *reinterpret_cast<uint4*>(pg + a.F) = make_uint4(wu[i][0], wu[i][1], wu[i][2], wu[i][3]);
+      const uint4 g4 = mx_tile_row(buf, i), d4 = mx_tile_row(buf + MX_TILE_BYTES, i), u4 = mx_tile_row(buf + 2 * MX_TILE_BYTES, i);
+      const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x2_t act, grad;
+        gated_act_grad2<kAct>(bf16x2_to_f32x2(g[j]), act, grad);
+        const f32x2_t d2 = bf16x2_to_f32x2(d[j]);
+        wu[i][j] = f32x2_to_bf16x2(mul2(d2, act));
+        wg[i][j] = f32x2_to_bf16x2(mul2(mul2(d2, bf16x2_to_f32x2(u[j])), grad));
       }
-      pg += 2 * a.F;
+      if (kCopies ? i % 4 == 3 : i % 3 == 2) __syncwarp();   // (where nothing spills)
     }
-  }
-  if (kDgu && a.amax != nullptr) {
-    const bool in = c0 + (lane & 7) * 8 < a.F;   // a tile across the border holds the first columns of u as g
-    uint32_t am = 0;
+    mx_release_tile(&empty[warp], ph, &abort_flag, a.status);
+    if (lane == 0 && tile + (int)gridDim.x < a.tiles) fetch(tile + gridDim.x);
+    if (kDgu && a.dgu != nullptr) {
+      const int64_t row = row0 + (lane >> 3) * 8, f = c0 + (lane & 7) * 8;
+      const int nrow = f < a.F ? mx_valid_rows(a.rows, row) : 0;
+      __nv_bfloat16* pg = a.dgu + row * 2 * a.F + f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) am = absmax2(am, absmax2(wu[i][j], wg[i][j]));
-    const uint32_t bits = __reduce_max_sync(0xffffffffu, in ? __float_as_uint(absmax2_to_float(am)) : 0u);
-    if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
-  }
-  if (!kCopies) continue;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    const MxTileScales sc = p ? mx_tile_store<kRagged>(o, wu, row0, a.F + c0, 2 * a.F)
-                              : mx_tile_store<kRagged>(o, wg, row0, c0, a.F);
-    const int r = wr * 32 + (lane >> 3) * 8 + (lane & 3) * 2, kb = wc * 2 + ((lane & 7) >> 2);
-    const int c = wc * 64 + (lane & 7) * 8 + (lane >> 3) * 2;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s_row[p][r + j][kb] = static_cast<uint8_t>(sc.row[j]);
-      s_col[p][c + j][wr] = static_cast<uint8_t>(sc.col[j]);
+      for (int i = 0; i < 8; ++i) {
+        if (i < nrow) {
+          *reinterpret_cast<uint4*>(pg) = make_uint4(wg[i][0], wg[i][1], wg[i][2], wg[i][3]);
+          *reinterpret_cast<uint4*>(pg + a.F) = make_uint4(wu[i][0], wu[i][1], wu[i][2], wu[i][3]);
+        }
+        pg += 2 * a.F;
+      }
     }
-  }
-  __syncthreads();
-  const uint32_t t = tid & 127;
-  if (tid < 128) {
-    const uint32_t r = (uint32_t)m0 + t;
-    const int n = (int)min((int64_t)4, (a.F - f0) >> 5);
+    if (kDgu && a.amax != nullptr) {
+      const bool in = c0 + (lane & 7) * 8 < a.F;   // a tile across the border holds the first columns of u as g
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) am = absmax2(am, absmax2(wu[i][j], wg[i][j]));
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, in ? __float_as_uint(absmax2_to_float(am)) : 0u);
+      if (lane == 0 && bits != 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), bits);
+    }
+    if (!kCopies) continue;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const uint32_t b0 = (uint32_t)((p ? a.F + f0 : f0) >> 5);
-      mx_store_scale_word(*reinterpret_cast<const uint32_t*>(s_row[p][t]), n, n == 4 && (b0 & 3) == 0 && row_words,
-                          r < o.rows ? o.s + (r * o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
-    }
-  } else if (o.q_t != nullptr && f0 + t < a.F) {
-    const uint32_t b0 = (uint32_t)(m0 >> 5);
-    const int n = (int)min((int64_t)4, ((o.rows + 31) >> 5) - b0);
+      const MxTileScales sc = p ? mx_tile_store<kRagged>(o, wu, row0, a.F + c0, 2 * a.F)
+                                : mx_tile_store<kRagged>(o, wg, row0, c0, a.F);
+      const int r = wr * 32 + (lane >> 3) * 8 + (lane & 3) * 2, kb = wc * 2 + ((lane & 7) >> 2);
+      const int c = wc * 64 + (lane & 7) * 8 + (lane >> 3) * 2;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const uint32_t c = (uint32_t)((p ? a.F : 0) + f0) + t, word = *reinterpret_cast<const uint32_t*>(s_col[p][t]);
-      mx_store_scale_word(word, n, n == 4 && col_words, o.s_t + (c * o.s_t_stride + b0), nullptr, c, b0, 0);
-      // (token blocks without a row: zeros)
-      if (o.s_t_swz != nullptr) *reinterpret_cast<uint32_t*>(o.s_t_swz + mx_swz_offset(c, b0, (uint32_t)o.kc_col)) = word;
+      for (int j = 0; j < 2; ++j) {
+        s_row[p][r + j][kb] = static_cast<uint8_t>(sc.row[j]);
+        s_col[p][c + j][wr] = static_cast<uint8_t>(sc.col[j]);
+      }
     }
-  }
-  // padding of the GEMM-layout scales: beyond the last feature, and token blocks up to the padded count
-  const int64_t mb0 = m0 >> 5, f1 = min(f0 + 128, a.F);
-  const bool last_x = tx == a.tiles_x - 1, last_y = (ty + 1) * a.tiles_x >= a.tiles;
-  if (last_x) {
-    mx_pad_row_scales(o, m0, 128, tid, 256);
-    for (int i = 0; i < 4; ++i) mx_pad_col_features(o, mb0 + i, tid, 256);
-  }
-  if (last_y) {
-    mx_pad_col_blocks(o, mb0 + 4, f0, f1, tid, 256);
-    mx_pad_col_blocks(o, mb0 + 4, a.F + f0, a.F + f1, tid, 256);
-    if (last_x) mx_pad_col_blocks(o, mb0 + 4, 2 * a.F, (2 * a.F + 127) / 128 * 128, tid, 256);
-  }
+    __syncthreads();
+    const uint32_t t = tid & 127;
+    if (tid < 128) {
+      const uint32_t r = (uint32_t)m0 + t;
+      const int n = (int)min((int64_t)4, (a.F - f0) >> 5);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t b0 = (uint32_t)((p ? a.F + f0 : f0) >> 5);
+        mx_store_scale_word(*reinterpret_cast<const uint32_t*>(s_row[p][t]), n, n == 4 && (b0 & 3) == 0 && row_words,
+                            r < o.rows ? o.s + (r * o.s_stride + b0) : nullptr, o.s_swz, r, b0, (uint32_t)o.kc_row);
+      }
+    } else if (o.q_t != nullptr && f0 + t < a.F) {
+      const uint32_t b0 = (uint32_t)(m0 >> 5);
+      const int n = (int)min((int64_t)4, ((o.rows + 31) >> 5) - b0);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t c = (uint32_t)((p ? a.F : 0) + f0) + t, word = *reinterpret_cast<const uint32_t*>(s_col[p][t]);
+        mx_store_scale_word(word, n, n == 4 && col_words, o.s_t + (c * o.s_t_stride + b0), nullptr, c, b0, 0);
+        // (token blocks without a row: zeros)
+        if (o.s_t_swz != nullptr) *reinterpret_cast<uint32_t*>(o.s_t_swz + mx_swz_offset(c, b0, (uint32_t)o.kc_col)) = word;
+      }
+    }
+    // padding of the GEMM-layout scales: beyond the last feature, and token blocks up to the padded count
+    const int64_t mb0 = m0 >> 5, f1 = min(f0 + 128, a.F);
+    const bool last_x = tx == a.tiles_x - 1, last_y = (ty + 1) * a.tiles_x >= a.tiles;
+    if (last_x) {
+      mx_pad_row_scales(o, m0, 128, tid, 256);
+      for (int i = 0; i < 4; ++i) mx_pad_col_features(o, mb0 + i, tid, 256);
+    }
+    if (last_y) {
+      mx_pad_col_blocks(o, mb0 + 4, f0, f1, tid, 256);
+      mx_pad_col_blocks(o, mb0 + 4, a.F + f0, a.F + f1, tid, 256);
+      if (last_x) mx_pad_col_blocks(o, mb0 + 4, 2 * a.F, (2 * a.F + 127) / 128 * 128, tid, 256);
+    }
   }
   pdl_trigger();
 }

@@ -363,10 +363,10 @@ __global__ void __launch_bounds__(32 * RN_PANEL_WARPS, 2)
     const float rstd_l = live ? rstd_of(total, a.cols, a.eps) : 0.0f;
     if (rank == 0 && warp == 0 && a.rstd != nullptr && live) a.rstd[row0 + lane] = rstd_l;
     if (w_ok) {
-  float g[8];
+      float g[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) g[k] = 0.0f;
-  if (c < a.cols) load_gamma8(a.gamma, a.gamma_f32, c, g);
+      for (int k = 0; k < 8; ++k) g[k] = 0.0f;
+      if (c < a.cols) load_gamma8(a.gamma, a.gamma_f32, c, g);
       uint32_t yw[8][4];
 #pragma unroll
       for (int i = 0; i < 8; ++i)    // (rows beyond the last are zeros)
