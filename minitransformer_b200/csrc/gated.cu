@@ -1,9 +1,9 @@
 // Gradient of the gated activation: from dh and the saved projections [g | u],
 //   du = bf16(dh * act(g)),   dg = bf16(dh * u * act'(g))
 // and, from the same registers, the MXFP8 copies of [dg | du] that the dgrad and wgrad GEMMs read (row-wise and
-// transposed). 6 bytes read and 4 written per (row, feature): bound by HBM. 8192 x 14336 with both copies takes 238 us (silu)
-// or 232 us (gelu) (1204 MB, 5.1 - 5.2 TB/s), the bf16 gradient alone 203 us (1174 MB, 5.8 TB/s; the same without the
-// arithmetic: 203 us, without the stores 101 us). 1021 x 1376: 12.4 us (1024 x 1376: 7.5 us).
+// transposed). 6 bytes read and 4 written per (row, feature): bound by HBM. 8192 x 14336 with both copies takes 236 us (silu)
+// or 233 us (gelu) (1204 MB, 5.1 - 5.2 TB/s), the bf16 gradient and its abs-max 207 or 212 us (1174 MB, 5.5 - 5.7 TB/s; without
+// the abs-max and the arithmetic 203 us, without the stores 101 us). 1021 x 1376: 12.2 / 12.5 us (1024 x 1376: 9.3 / 9.4 us).
 #include "gated_act.cuh"
 #include "tile_quant.cuh"
 

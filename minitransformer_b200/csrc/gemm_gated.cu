@@ -17,8 +17,9 @@
 //
 // gemm_gated_pair_kernel (the rest): a CTA pair (cta_group::2) per 256 rows x 128 features. The B tile of
 // 256 rows is [128 rows of Wg; 128 rows of Wu], one half loaded by either CTA, so g and u of a feature end up 128
-// accumulator columns apart in the same lane. Bound by the tensor pipe (89 % busy in the NVFP4 form): 8192 x 4096 x 14336
-// takes 342 us (NVFP4, 5.6 PFLOP/s) or 645 us (MXFP8, 3.0) for h alone, 392 and 681 with [g | u] as well.
+// accumulator columns apart in the same lane. Bound by the tensor pipe (82 % busy in the NVFP4 form, 74 % when it writes
+// [g | u] as well, 89 % in the MXFP8 form) and by power: 8192 x 4096 x 14336 takes 342 us (NVFP4, 5.6 PFLOP/s) or 645 us
+// (MXFP8, 3.0) for h alone, 392 and 681 with [g | u]; twenty in a row, at the power cap, 350, 750, 410 and 770 us each.
 //
 // Every wait on an mbarrier is bounded, as in the plain GEMM kernels.
 #include <algorithm>

@@ -728,7 +728,8 @@ static int rn_threads(int64_t cols, int V) { return (int)(((cols / 8 + V - 1) / 
 // CTAs per SM that share its memory for their rings, one vector of 8 columns per thread: two CTAs of 512 threads on
 // 4096 columns, one of 1024 on 8192. With two vectors per thread (two CTAs of 512) the gradient of 8192 x 8192 took
 // 119 us instead of 84. Beyond 8192 columns four vectors per thread of one CTA of 512: 4096 x 16384 takes 118 us with a
-// residual and 89 without (4.5 TB/s), 126 and 110 us with two vectors per thread of 1024, which leave it 64 registers.
+// residual and 89 without (4.5 TB/s), though 124 bytes of it spill; 126 and 110 us with two vectors per thread of 1024, which
+// leave it 64 registers.
 static int rn_ring_ctas_per_sm(int64_t cols) { return cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1; }
 static int rn_ring_stages(int64_t cols, int64_t stage) {
   const int64_t n = RN_RING_BYTES / rn_ring_ctas_per_sm(cols) / stage;
