@@ -104,14 +104,20 @@ class QuantizeResultCache:
 
 
 class TensorCopies:
-    """Quantized copies that the producer of a tensor made along with it. They hang on that tensor and go when it does,
-    so that a module which remembers this object keeps no memory alive, and they count for that tensor alone, as long
-    as it has not been changed in place (changes made in inference mode go unnoticed: torch does not count them)."""
+    """Quantized copies that the producer of a tensor made along with it. They go when that tensor goes, so that a module
+    which remembers this object keeps no memory alive, and they count for that tensor alone, as long as it has not
+    been changed in place (changes made in inference mode go unnoticed: torch does not count them)."""
 
     def __init__(self, tensor: torch.Tensor, copies: QuantizeResult) -> None:
-        tensor._mt_copies = copies
-        self.shape = tuple(copies.data.shape)
-        self._tensor = weakref.ref(tensor)
+        holder = weakref.ref(self)
+
+        def gone(_):
+            me = holder()
+            if me is not None:
+                me._copies = None
+
+        self.shape, self._copies = tuple(copies.data.shape), copies
+        self._tensor = weakref.ref(tensor, gone)
         self._version = None if tensor.is_inference() else tensor._version
 
     def of(self, x: torch.Tensor) -> Optional[QuantizeResult]:
@@ -121,7 +127,7 @@ class TensorCopies:
             return None
         if self._version is not None and tensor._version != self._version:
             return None
-        return tensor._mt_copies
+        return self._copies
 
     def __reduce__(self):
         return _gone_copies, (self.shape,)       # a copied or unpickled module remembers no tensor
@@ -129,7 +135,7 @@ class TensorCopies:
 
 def _gone_copies(shape) -> TensorCopies:
     c = TensorCopies.__new__(TensorCopies)
-    c.shape, c._tensor, c._version = shape, (lambda: None), None
+    c.shape, c._copies, c._tensor, c._version = shape, None, (lambda: None), None
     return c
 
 

@@ -27,8 +27,31 @@ def test_copies_live_as_long_as_their_tensor():
     del made
     assert alive() is not None
     del y
-    gc.collect()
     assert alive() is None and t.of(torch.zeros(32, 64, dtype=torch.bfloat16)) is None
+
+
+def test_copies_leave_no_trace_on_their_tensor(tmp_path):
+    y = torch.zeros(32, 64, dtype=torch.bfloat16)
+    t = Q.TensorCopies(y, _copies(32, 64))
+    torch.save(y, tmp_path / "y.pt")
+    assert torch.equal(torch.load(tmp_path / "y.pt", weights_only=True), y) and t.of(y) is not None
+    alive = weakref.ref(t.of(y).data)
+    del t                                                    # the layer's next call
+    assert alive() is None
+
+
+def test_copies_of_a_tensor_that_only_autograd_holds():
+    """The tensor's Python object goes and comes back while a graph holds it; the copies go with the graph."""
+    w = torch.ones(32, 64, requires_grad=True)
+    y = torch.zeros(32, 64)
+    t = Q.TensorCopies(y, _copies(32, 64))
+    alive = weakref.ref(t.of(y).data)
+    out = (y * w).sum()                                      # saves y
+    del y
+    out.backward()
+    del out
+    gc.collect()
+    assert alive() is None
 
 
 def test_copies_count_for_their_tensor_unchanged():
